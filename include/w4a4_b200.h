@@ -318,6 +318,81 @@ int w4a4_fused_dense_sparse_noalloc(const void* W_low, const void* W_high, const
                                     const void* zero_u4, const int32_t* sum_X, const void* scale_x, void* Y,
                                     int T, int K, int N, int nnz, int flags, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Operators on a paged key/value cache: what stands between the qkv linear and the o linear of a decoder layer.  No
+ * counterpart in the reference's bindings (its layer harness is PyTorch, bench/layer/qwen3_layer_bf16.py:129-241).
+ *
+ * Pages: k_pages and v_pages hold n_pages pages of page_size slots (a multiple of 16) for each key/value head; element
+ * (page, head, slot, d) is at page * strides[0] + head * strides[1] + slot * strides[2] + d, strides in elements,
+ * positive and multiples of 8, pointers 16-byte aligned, head_dim 64 or 128.  Slot j of sequence b is slot
+ * j % page_size of page block_table[b * table_stride + j / page_size].
+ * Sequences: cu_seqlens (n_seqs + 1) int32 holds the first token of each sequence and the end of the last; lengths
+ * (n_seqs) int32 counts the cache slots in use, those of the call's new tokens included.  New token i of sequence b
+ * has slot lengths[b] - q_len[b] + i and sees the slots up to its own.  Both are device memory, like block_table, and
+ * no host check sees their values: what is out of range (a page number, a length beyond max_pages * page_size, offsets
+ * that do not rise, more new tokens than max_q_len, a position outside the tables) is cut to what is in range, reads
+ * zeros or is left out, and sets the device error word (w4a4_device_error).  A sequence may have no new token; tokens
+ * behind the last sequence are neither read nor written. */
+#define W4A4_F16  0
+#define W4A4_BF16 1
+typedef struct w4a4_paged_kv {
+  void* k_pages;
+  void* v_pages;
+  long long k_strides[3];        /* page, head, slot; elements */
+  long long v_strides[3];
+  const int32_t* block_table;    /* (n_seqs, max_pages), row stride table_stride */
+  long long table_stride;
+  int n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages;
+  int dtype;                     /* W4A4_F16 or W4A4_BF16: pages, queries, outputs, norm weights */
+} w4a4_paged_kv;
+
+/* From the output of the qkv linear, qkv (T, (n_heads + 2 * n_kv_heads) * head_dim) with row stride ld_qkv (queries,
+ * keys, values): norm of every query and key head x * w / sqrt(mean(x^2) + eps) where a weight (head_dim) is given,
+ * rotation (a, b) -> (a c - b s, b c + a s) of the first rot_dim elements (a multiple of 16; pairs are neighbours when
+ * interleaved, else i and i + rot_dim / 2), queries to q_out (T, n_heads, head_dim), keys and values to their cache
+ * slots.  cos and sin (max_pos, rot_dim / 2) float; a token's position is its slot, plus offsets[b] where offsets is
+ * given (slots that were evicted).  One rounding per value.  q_out may be the query columns of qkv. */
+int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long ld_qkv, const int32_t* cu_seqlens,
+                        const int32_t* lengths, const float* cos, const float* sin, int max_pos, int rot_dim,
+                        const void* q_norm, const void* k_norm, float eps, int interleaved, const int32_t* offsets,
+                        void* q_out, long long q_tok_stride, long long q_head_stride, int T, int n_heads, void* stream);
+
+/* out[t, h] = sum_j softmax_j(scale * q[t, h] . k[j]) v[j] over the slots j that new token t sees, key/value head
+ * h / (n_heads / n_kv_heads).  A token that sees no slot (its own would be negative) gets zeros.  lse (T, n_heads)
+ * float, or NULL: natural logarithm of the sum of exponentials, minus infinity where nothing is seen.  Values in slots
+ * that a token does not see must be finite up to its sequence's length (a weight of zero times infinity is NaN);
+ * beyond the length they may hold anything.  max_q_len: no sequence has more new tokens.
+ * workspace: w4a4_paged_attention_workspace_bytes (0: an argument is bad), 16-byte aligned; its first
+ * W4A4_ATTENTION_STATE_BYTES must be zero before the first call and are zero again after each; calls that share it
+ * must be ordered on one stream.  It is not the workspace of the linears. */
+#define W4A4_ATTENTION_STATE_BYTES 4096
+size_t w4a4_paged_attention_workspace_bytes(const w4a4_paged_kv* cache, int T, int n_heads, int max_q_len);
+int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
+                         const int32_t* cu_seqlens, const int32_t* lengths, void* out, long long out_tok_stride,
+                         long long out_head_stride, float* lse, int T, int n_heads, int max_q_len, float scale,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* Adds to sums[b, g, j] the attention weight that slot j of sequence b has received from the call's new tokens:
+ * sum over the new tokens i that see j and the heads h of group g of exp(scale * q[i, h] . k[j] - lse[i, h]), lse from
+ * w4a4_paged_attention.  sums: float, row strides in elements, max_pages * page_size (at least) floats a row; slots
+ * beyond a sequence's length are not touched. */
+int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
+                           const int32_t* cu_seqlens, const int32_t* lengths, const float* lse, float* sums,
+                           long long sums_seq_stride, long long sums_head_stride, int T, int n_heads, int max_q_len,
+                           float scale, void* stream);
+
+/* Keeps, for every sequence and key/value head on its own, n_sink first slots, n_recent last ones and those with the
+ * largest sums in between, `budget` in all (equal sums: the lowest slots first; NaN counts as the least), and moves
+ * them in their order to the slots 0, 1, ... of `into`, which is `cache` itself (in place) or another cache of the same
+ * sequences, heads, head_dim and dtype.  Two caches may share pages only where slot j of a sequence is the same memory
+ * in both, and no two sequences may share pages that are moved.  kept (n_seqs, n_kv_heads, budget): old slot of each new one,
+ * -1 behind the last; new_lengths (n_seqs) = min(length, budget); new_sums (n_seqs, n_kv_heads, into's max_pages *
+ * page_size), zero behind the last slot; none of them may overlap an input.  Slots of `into` behind new_lengths keep
+ * what they held. */
+int w4a4_cache_evict(const w4a4_paged_kv* cache, const w4a4_paged_kv* into, const int32_t* lengths, const float* sums,
+                     long long sums_seq_stride, long long sums_head_stride, int budget, int n_sink, int n_recent,
+                     int32_t* kept, int32_t* new_lengths, float* new_sums, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

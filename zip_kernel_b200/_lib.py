@@ -60,7 +60,20 @@ SIGNATURES = {
     "w4a4_expand_activations_fmt": (_INT, [_PTR] * 4 + [_INT, _INT, _INT, _PTR]),
     "w4a4_fused_dense_sparse_expanded_prepared": (_INT, [_PTR] * 12 + [_INT] * 5 + [_PTR, _SZ, _PTR]),
     "w4a4_dump_accumulators_prepared": (_INT, [_PTR] * 9 + [_INT] * 5 + [_PTR, _SZ, _PTR]),
+    "w4a4_qkv_rope_cache": (_INT, [_PTR, _PTR, _LL] + [_PTR] * 4 + [_INT, _INT, _PTR, _PTR, _c.c_float, _INT, _PTR, _PTR, _LL, _LL, _INT, _INT, _PTR]),
+    "w4a4_paged_attention_workspace_bytes": (_SZ, [_PTR, _INT, _INT, _INT]),
+    "w4a4_paged_attention": (_INT, [_PTR, _PTR, _LL, _LL, _PTR, _PTR, _PTR, _LL, _LL, _PTR, _INT, _INT, _INT, _c.c_float, _PTR, _SZ, _PTR]),
+    "w4a4_cache_weight_sums": (_INT, [_PTR, _PTR, _LL, _LL] + [_PTR] * 4 + [_LL, _LL, _INT, _INT, _INT, _c.c_float, _PTR]),
+    "w4a4_cache_evict": (_INT, [_PTR] * 4 + [_LL, _LL, _INT, _INT, _INT] + [_PTR] * 4),
 }
+
+
+class PagedKVArg(_c.Structure):
+    """``w4a4_paged_kv`` of include/w4a4_b200.h."""
+    _fields_ = [("k_pages", _PTR), ("v_pages", _PTR), ("k_strides", _LL * 3), ("v_strides", _LL * 3), ("block_table", _PTR),
+                ("table_stride", _LL), ("n_pages", _INT), ("page_size", _INT), ("n_kv_heads", _INT), ("head_dim", _INT),
+                ("n_seqs", _INT), ("max_pages", _INT), ("dtype", _INT)]
+
 
 FLAG_OUT_TOKEN_MAJOR = 0x1
 FLAG_FORCE_STREAM = 0x2
@@ -70,6 +83,8 @@ FLAG_CODES_E4M3_PACKED = 0x10
 FLAG_TILES_128 = 0x20
 FLAG_TILES_256 = 0x40
 CODES_S8, CODES_E4M3, CODES_E4M3_PACKED = 0, 1, 2
+F16, BF16 = 0, 1
+ATTENTION_STATE_BYTES = 4096
 KERNEL_STREAM, KERNEL_TILES_128, KERNEL_TILES_256, KERNEL_PAIRS = 0, 1, 2, 3
 
 _lib = None
@@ -154,7 +169,7 @@ def on_device(device):
 # memory.  Code that captures wraps warm-up and capture in
 # ``use_workspace(holder)`` and keeps ``holder`` alive next to the graph.
 # ---------------------------------------------------------------------------
-_workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
+_workspaces: Dict[tuple, torch.Tensor] = {}
 _tls = threading.local()
 
 
@@ -164,9 +179,9 @@ class WorkspaceHolder:
     captured kernel may reference is never freed or replaced while the holder lives."""
 
     def __init__(self):
-        self.buffers: Dict[Tuple[int, int], list] = {}
+        self.buffers: Dict[tuple, list] = {}
 
-    def get(self, key: Tuple[int, int], need: int, device: torch.device) -> torch.Tensor:
+    def get(self, key: tuple, need: int, device: torch.device) -> torch.Tensor:
         bufs = self.buffers.setdefault(key, [])
         if bufs and bufs[-1].numel() >= need:
             return bufs[-1]
@@ -176,6 +191,8 @@ class WorkspaceHolder:
                 "run the shape once eagerly inside use_workspace(holder) first"
             )
         buf = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+        if len(key) > 2:
+            buf[:ATTENTION_STATE_BYTES].zero_()
         bufs.append(buf)
         return buf
 
@@ -211,6 +228,25 @@ def workspace(device: torch.device, T: int, K: int, N: int, nnz: int) -> torch.T
             )
         grow = max(need, int(buf.numel() * 1.5) if buf is not None else 0)
         buf = torch.empty(grow, dtype=torch.uint8, device=device)
+        _workspaces[key] = buf
+    return buf
+
+
+def attention_workspace(kv, T: int, n_heads: int, max_q_len: int) -> torch.Tensor:
+    """Scratch of the attention on a paged cache: apart from the linears' because its counters start, and end, as zeros."""
+    need = int(load().w4a4_paged_attention_workspace_bytes(kv._ptr, T, n_heads, max_q_len))
+    key = (kv.device.index, stream_ptr(kv.device), "attention")
+    holder = getattr(_tls, "holder", None)
+    if holder is not None:
+        return holder.get(key, need, kv.device)
+    buf = _workspaces.get(key)
+    if buf is None or buf.numel() < need:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(
+                "the attention workspace must be allocated before CUDA-graph capture: run the shape once eagerly on this stream"
+            )
+        buf = torch.empty(need, dtype=torch.uint8, device=kv.device)
+        buf[:ATTENTION_STATE_BYTES].zero_()
         _workspaces[key] = buf
     return buf
 

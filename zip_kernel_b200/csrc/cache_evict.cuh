@@ -1,0 +1,210 @@
+// Eviction from a paged cache by accumulated weight: for each sequence and key/value head the first `sink` slots, the
+// last `recent` ones and those with the largest sums in between, `budget` in all (equal sums: the lowest slots), move in
+// their order to the slots 0, 1, ... of the destination.  A sequence of at most `budget` slots keeps them all.
+//
+// Two launches.  select: a block per (sequence, head) finds the smallest sum that stays by a radix selection, eight bits
+// of an order-preserving integer form of the float at a time, then walks the slots once in order and writes the list of
+// those kept and their sums.  move: copies the rows of the list.  In place a row's new slot is never above its old one,
+// so rows may be written in ascending order once all rows up to them have been read; the columns of a row are
+// independent of one another, and a block takes a few columns of all rows of one (sequence, head).  Into another cache
+// the rows are independent too and are split over blocks.
+//
+// What bounds it: the rows kept are read and written once; the selection reads the sums six times, from L2 after the first.
+#pragma once
+
+#include "paged_kv.cuh"
+
+namespace w4a4 {
+namespace evict {
+
+using namespace kv;
+
+constexpr int SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, BINS = 256;
+constexpr int MOVE_THREADS = 256, MOVE_UNROLL = 4;
+
+struct SelectParams {
+  const int32_t* lengths;
+  const float* sums;
+  long long sums_seq, sums_head;
+  int32_t* kept;              // (n_seqs, n_kv, budget)
+  int32_t* new_lengths;
+  float* new_sums;            // (n_seqs, n_kv, new_slots)
+  int n_kv, max_slots, new_slots, budget, sink, recent;
+};
+
+// Unsigned integers in the order of the floats: both zeros alike, NaN below everything.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (!(x == x)) return 0;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const SelectParams p) {
+  __shared__ int hist[SELECT_WARPS][BINS];
+  __shared__ int warp_sums[2][SELECT_WARPS];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_left;
+  grid_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.x / p.n_kv, g = blockIdx.x % p.n_kv;
+  grid_dependency_wait();
+  const int len = ld_plain(p.lengths + b), n = min(max(len, 0), p.max_slots);
+  if (n != len && tid == 0) record_error(SITE_KV_SEQ, b);
+  const int n_new = min(n, p.budget);
+  if (g == 0 && tid == 0) p.new_lengths[b] = n_new;
+  const float* sums = p.sums + (long long)b * p.sums_seq + (long long)g * p.sums_head;
+  int32_t* kept = p.kept + ((long long)b * p.n_kv + g) * p.budget;
+  float* out = p.new_sums + ((long long)b * p.n_kv + g) * p.new_slots;
+
+  if (n <= p.budget) {
+    for (int j = tid; j < n; j += SELECT_THREADS) {
+      kept[j] = j;
+      out[j] = ld_plain(sums + j);
+    }
+  } else {
+    const int lo = p.sink, hi = n - p.recent;              // candidates; the rest stays anyway (sink + recent <= budget < n)
+    int left = p.budget - p.sink - p.recent;               // how many of them stay
+    uint32_t prefix = 0;                                   // leading bits of the smallest key that stays
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < SELECT_WARPS * BINS; i += SELECT_THREADS) hist[i / BINS][i % BINS] = 0;
+      __syncthreads();
+      for (int j = lo + tid; j < hi; j += SELECT_THREADS) {
+        const uint32_t k = order_key(ld_plain(sums + j));
+        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[warp][(k >> shift) & 255], 1);
+      }
+      __syncthreads();
+      if (tid < BINS) {
+        int s = 0;
+        for (int k = 0; k < SELECT_WARPS; ++k) s += hist[k][tid];
+        hist[0][tid] = s;
+      }
+      __syncthreads();
+      if (warp == 0) {
+        // bins from the top: the one in which the count reaches `left`
+        int mine[8], s = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { mine[i] = hist[0][255 - (lane * 8 + i)]; s += mine[i]; }
+        int above = s;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const int a = __shfl_up_sync(0xffffffffu, above, o);
+          if (lane >= o) above += a;
+        }
+        above -= s;                                        // of the lanes before
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (above < left && left <= above + mine[i]) {
+            s_prefix = prefix | ((uint32_t)(255 - (lane * 8 + i)) << shift);
+            s_left = left - above;
+          }
+          above += mine[i];
+        }
+      }
+      __syncthreads();
+      if (left > 0) { prefix = s_prefix; left = s_left; }
+    }
+    // Now `prefix` is the smallest key that stays, `left` how many slots with just that key do: the first ones.
+    const bool any = p.budget > p.sink + p.recent;
+    int done = 0, ties = 0;                                // slots kept, and slots with that key, before this round
+    for (int base = 0; base < n; base += SELECT_THREADS) {
+      const int j = base + tid;
+      bool sure = false, tie = false;
+      float v = 0.f;
+      if (j < n) {
+        v = ld_plain(sums + j);
+        const uint32_t k = order_key(v);
+        const bool free = j >= lo && j < hi;
+        sure = !free || (any && k > prefix);
+        tie = free && any && k == prefix;
+      }
+      const unsigned ms = __ballot_sync(0xffffffffu, sure), mt = __ballot_sync(0xffffffffu, tie), before = (1u << lane) - 1;
+      if (lane == 0) { warp_sums[0][warp] = __popc(ms); warp_sums[1][warp] = __popc(mt); }
+      __syncthreads();
+      const int ws = warp_sums[0][lane], wt = warp_sums[1][lane];
+      const int s_before = __reduce_add_sync(0xffffffffu, lane < warp ? ws : 0) + __popc(ms & before);
+      const int t_before = ties + __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0) + __popc(mt & before);
+      const int s_all = __reduce_add_sync(0xffffffffu, ws), t_all = __reduce_add_sync(0xffffffffu, wt);
+      if (sure || (tie && t_before < left)) {
+        const int to = done + s_before + min(t_before, left) - min(ties, left);
+        kept[to] = j;
+        out[to] = v;
+      }
+      done += s_all + min(ties + t_all, left) - min(ties, left);
+      ties += t_all;
+      __syncthreads();
+    }
+  }
+  for (int j = n_new + tid; j < p.budget; j += SELECT_THREADS) kept[j] = -1;
+  for (int j = n_new + tid; j < p.new_slots; j += SELECT_THREADS) out[j] = 0.f;
+}
+
+struct MoveParams {
+  Cache from, to;
+  const int32_t* kept;
+  const int32_t* new_lengths;
+  int budget, chunks;         // 16-byte chunks of a row (keys then values) that a block takes
+  int parts, rows_per_part;   // blocks over the rows of one (sequence, head); one when the caches share memory
+  int in_place;
+};
+
+__global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const MoveParams p) {
+  grid_launch_dependents();
+  const int tid = threadIdx.x;
+  const int row_chunks = p.from.dim / 8;                   // of a key or value row
+  const int slices = 2 * row_chunks / p.chunks;
+  const int part = blockIdx.x % p.parts, rest = blockIdx.x / p.parts;
+  const int slice = rest % slices, unit = rest / slices;
+  const int b = unit / p.from.n_kv, g = unit % p.from.n_kv;
+  const int chunk = slice * p.chunks + tid % p.chunks;
+  const bool is_v = chunk >= row_chunks;
+  const int d = (is_v ? chunk - row_chunks : chunk) * 8;
+  const uint16_t* src = static_cast<const uint16_t*>(is_v ? p.from.v : p.from.k) + g * (is_v ? p.from.v_head : p.from.k_head) + d;
+  uint16_t* dst = static_cast<uint16_t*>(is_v ? p.to.v : p.to.k) + g * (is_v ? p.to.v_head : p.to.k_head) + d;
+  const long long s_page = is_v ? p.from.v_page : p.from.k_page, s_slot = is_v ? p.from.v_slot : p.from.k_slot;
+  const long long d_page = is_v ? p.to.v_page : p.to.k_page, d_slot = is_v ? p.to.v_slot : p.to.k_slot;
+  const int rows = MOVE_THREADS / p.chunks, batch = rows * MOVE_UNROLL;
+  grid_dependency_wait();
+  const int n = min(ld_plain(p.new_lengths + b), p.budget);
+  const int first = part * p.rows_per_part, end = min(n, first + p.rows_per_part);
+  const int32_t* kept = p.kept + (long long)unit * p.budget;
+
+  uint4 x[2][MOVE_UNROLL];
+  bool live[2][MOVE_UNROLL];
+  auto load = [&](int k, int row0) {
+#pragma unroll
+    for (int u = 0; u < MOVE_UNROLL; ++u) {
+      const int i = row0 + u * rows + tid / p.chunks;
+      live[k][u] = i < end;
+      if (!live[k][u]) continue;
+      const int j = ld_plain(kept + i);
+      if (p.in_place && j == i) { live[k][u] = false; continue; }
+      const int page = page_of(p.from, b, j / p.from.page);
+      live[k][u] = page >= 0;
+      if (page >= 0) x[k][u] = ld_plain(reinterpret_cast<const uint4*>(src + page * s_page + (j % p.from.page) * s_slot));
+    }
+  };
+  auto store = [&](int k, int row0) {
+#pragma unroll
+    for (int u = 0; u < MOVE_UNROLL; ++u) {
+      const int i = row0 + u * rows + tid / p.chunks;
+      if (!live[k][u]) continue;
+      const int page = page_of(p.to, b, i / p.to.page);
+      if (page >= 0) *reinterpret_cast<uint4*>(dst + page * d_page + (i % p.to.page) * d_slot) = x[k][u];
+    }
+  };
+  // The rows of a batch are stored once every thread has loaded its own; those of the next may be loaded before,
+  // they lie at or above the batch's end.
+  if (first >= end) return;
+  load(0, first);
+  for (int row0 = first; row0 < end; row0 += 2 * batch) {
+    load(1, row0 + batch);
+    __syncthreads();
+    store(0, row0);
+    load(0, row0 + 2 * batch);
+    __syncthreads();
+    store(1, row0 + batch);
+  }
+}
+
+}  // namespace evict
+}  // namespace w4a4

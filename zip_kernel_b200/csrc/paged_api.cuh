@@ -1,0 +1,361 @@
+// Entry points of the operators on a paged key/value cache: argument checks, tensor maps and launches.
+// Included by w4a4_lib.cu, whose helpers it uses.
+#pragma once
+
+namespace {
+
+namespace kv = w4a4::kv;
+namespace pdec = w4a4::pdec;
+namespace csum = w4a4::csum;
+namespace evict = w4a4::evict;
+
+int check_cache(const w4a4_paged_kv* c) {
+  CHECK_ARG(c != nullptr, "cache is NULL");
+  CHECK_ARG(c->dtype == W4A4_F16 || c->dtype == W4A4_BF16, "cache dtype %d is neither W4A4_F16 nor W4A4_BF16", c->dtype);
+  CHECK_ARG(c->head_dim == 64 || c->head_dim == 128, "head_dim must be 64 or 128, got %d", c->head_dim);
+  CHECK_ARG(c->page_size >= 16 && c->page_size % 16 == 0, "page_size must be a positive multiple of 16, got %d", c->page_size);
+  CHECK_ARG(c->n_kv_heads >= 1 && c->n_pages >= 1, "n_kv_heads %d and n_pages %d must be positive", c->n_kv_heads, c->n_pages);
+  CHECK_ARG(c->n_seqs >= 0 && c->max_pages >= 0, "n_seqs %d and max_pages %d must not be negative", c->n_seqs, c->max_pages);
+  CHECK_ARG((long long)c->max_pages * c->page_size < (1LL << 31) - 1024, "a sequence of %d pages of %d slots is too long",
+            c->max_pages, c->page_size);
+  CHECK_ARG(c->k_pages && c->v_pages && (c->block_table || c->n_seqs == 0 || c->max_pages == 0), "NULL cache pointer");
+  CHECK_ARG(c->table_stride >= c->max_pages, "table_stride (%lld) must be >= max_pages (%d)", c->table_stride, c->max_pages);
+  for (int i = 0; i < 3; ++i) {
+    CHECK_ARG(c->k_strides[i] > 0 && c->v_strides[i] > 0 && c->k_strides[i] < (1LL << 38) && c->v_strides[i] < (1LL << 38),
+              "cache strides must be positive and below 2^38 elements");
+    if (c->k_strides[i] % 8 || c->v_strides[i] % 8)
+      return fail(W4A4_ERR_ALIGNMENT, "cache strides must be multiples of 8 elements");
+  }
+  if (!aligned(c->k_pages, 16) || !aligned(c->v_pages, 16) || !aligned(c->block_table, 4))
+    return fail(W4A4_ERR_ALIGNMENT, "cache pointers must be 16-byte aligned");
+  return W4A4_OK;
+}
+
+kv::Cache device_cache(const w4a4_paged_kv* c) {
+  kv::Cache d;
+  d.k = c->k_pages;
+  d.v = c->v_pages;
+  d.k_page = c->k_strides[0]; d.k_head = c->k_strides[1]; d.k_slot = c->k_strides[2];
+  d.v_page = c->v_strides[0]; d.v_head = c->v_strides[1]; d.v_slot = c->v_strides[2];
+  d.table = c->block_table;
+  d.table_stride = c->table_stride;
+  d.n_pages = c->n_pages;
+  d.page = c->page_size;
+  d.n_kv = c->n_kv_heads;
+  d.dim = c->head_dim;
+  d.n_seqs = c->n_seqs;
+  d.max_pages = c->max_pages;
+  return d;
+}
+
+kv::Seqs device_seqs(const w4a4_paged_kv* c, const int32_t* cu, const int32_t* lengths, int T, int max_q) {
+  kv::Seqs s;
+  s.cu = cu;
+  s.lengths = lengths;
+  s.n = c->n_seqs;
+  s.T = T;
+  s.max_slots = c->max_pages * c->page_size;
+  s.max_q = max_q;
+  return s;
+}
+
+// Row strides of a (T, heads, dim) operand: the heads of a token do not overlap, nor do the tokens.
+int check_rows(const char* what, const void* ptr, long long tok, long long head, int T, int n_heads, int dim) {
+  CHECK_ARG(ptr != nullptr, "%s is NULL", what);
+  CHECK_ARG(head >= dim || n_heads == 1, "%s: head stride %lld is below head_dim %d", what, head, dim);
+  CHECK_ARG(tok >= dim || T == 1, "%s: token stride %lld is below head_dim %d", what, tok, dim);
+  if (!aligned(ptr, 16) || tok % 8 || head % 8)
+    return fail(W4A4_ERR_ALIGNMENT, "%s must be 16-byte aligned with strides that are multiples of 8 elements", what);
+  return W4A4_OK;
+}
+
+int check_seqs(const w4a4_paged_kv* c, const int32_t* cu, const int32_t* lengths, int T, int n_heads) {
+  CHECK_ARG(T >= 0, "T must not be negative, got %d", T);
+  CHECK_ARG(n_heads >= 1 && n_heads % c->n_kv_heads == 0, "n_heads (%d) must be a positive multiple of n_kv_heads (%d)", n_heads,
+            c->n_kv_heads);
+  CHECK_ARG(c->n_seqs == 0 || (cu && lengths), "cu_seqlens or lengths is NULL");
+  if (!aligned(cu, 4) || !aligned(lengths, 4)) return fail(W4A4_ERR_ALIGNMENT, "cu_seqlens and lengths must be 4-byte aligned");
+  return W4A4_OK;
+}
+
+// Slots of one copy box: the largest power of two up to `tile` that divides a page, so that no box leaves its page.
+int box_slots(int page, int tile) {
+  int b = page & -page;
+  return b < tile ? b : tile;
+}
+
+// 4-D map {element, slot, head, page} of keys or values, boxes of 64 elements x `box` slots, 128-byte swizzle.
+int make_cache_map(CUtensorMap* m, const w4a4_paged_kv* c, bool values, int box) {
+  const long long* st = values ? c->v_strides : c->k_strides;
+  cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->n_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
+  cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = g_encode(m, c->dtype == W4A4_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                        values ? c->v_pages : c->k_pages, dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(W4A4_ERR_LAUNCH, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return W4A4_OK;
+}
+
+// 3-D map {element, head, token} of queries, boxes of 64 elements x `heads` x `toks`, 128-byte swizzle: the rows of a
+// box lie token by token, in each the heads.
+int make_query_map(CUtensorMap* m, const void* q, long long tok, long long head, int T, int n_heads, int dim, int dtype, int heads, int toks) {
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)n_heads, (cuuint64_t)T};
+  cuuint64_t strides[2] = {(cuuint64_t)(n_heads == 1 ? dim : head) * 2, (cuuint64_t)(T == 1 ? (long long)n_heads * dim : tok) * 2};
+  cuuint32_t boxes[3] = {64, (cuuint32_t)heads, (cuuint32_t)toks};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(m, dtype == W4A4_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                        const_cast<void*>(q), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(W4A4_ERR_LAUNCH, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return W4A4_OK;
+}
+
+template <typename F16K, typename BF16K>
+auto by_type(int dtype, F16K a, BF16K b) { return dtype == W4A4_F16 ? a : b; }
+
+// ------------------------------------------------------------------ attention workspace: counters, then parts
+constexpr size_t ATTN_COUNTERS = W4A4_ATTENTION_STATE_BYTES / 4;
+
+}  // namespace
+
+extern "C" {
+
+int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long ld_qkv, const int32_t* cu_seqlens,
+                        const int32_t* lengths, const float* cos, const float* sin, int max_pos, int rot_dim,
+                        const void* q_norm, const void* k_norm, float eps, int interleaved, const int32_t* offsets,
+                        void* q_out, long long q_tok_stride, long long q_head_stride, int T, int n_heads, void* stream) {
+  begin_call();
+  int rc = check_cache(cache);
+  if (!rc) rc = check_seqs(cache, cu_seqlens, lengths, T, n_heads);
+  if (rc) return rc;
+  CHECK_ARG(rot_dim >= 0 && rot_dim <= cache->head_dim && rot_dim % 16 == 0, "rot_dim must be a multiple of 16 up to head_dim, got %d", rot_dim);
+  CHECK_ARG(rot_dim == 0 || (cos && sin), "cos or sin is NULL");
+  if (T == 0 || cache->n_seqs == 0) return W4A4_OK;
+  CHECK_ARG(qkv != nullptr, "qkv is NULL");
+  CHECK_ARG(T == 1 || ld_qkv >= (long long)(n_heads + 2 * cache->n_kv_heads) * cache->head_dim, "ld_qkv (%lld) is below the width of a row", ld_qkv);
+  rc = check_rows("q_out", q_out, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
+  if (rc) return rc;
+  if (!aligned(qkv, 16) || ld_qkv % 8 || !aligned(cos, 16) || !aligned(sin, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16))
+    return fail(W4A4_ERR_ALIGNMENT, "qkv, cos, sin and the norm weights must be 16-byte aligned");
+  DeviceInfo* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  kv::RopeParams p;
+  p.c = device_cache(cache);
+  p.s = device_seqs(cache, cu_seqlens, lengths, T, T);
+  p.qkv = qkv;
+  p.ld_qkv = ld_qkv;
+  p.q_out = q_out;
+  p.q_tok = q_tok_stride;
+  p.q_head = q_head_stride;
+  p.cos = cos;
+  p.sin = sin;
+  p.q_norm = q_norm;
+  p.k_norm = k_norm;
+  p.offsets = offsets;
+  p.n_heads = n_heads;
+  p.rot = rot_dim;
+  p.max_pos = max_pos;
+  p.interleaved = interleaved != 0;
+  p.eps = eps;
+  auto kern = cache->head_dim == 128 ? by_type(cache->dtype, kv::qkv_rope_kernel<__half, 128>, kv::qkv_rope_kernel<__nv_bfloat16, 128>)
+                                     : by_type(cache->dtype, kv::qkv_rope_kernel<__half, 64>, kv::qkv_rope_kernel<__nv_bfloat16, 64>);
+  cudaError_t e = launch_ex(kern, dim3((unsigned)T), dim3(kv::ROPE_THREADS), 0, static_cast<cudaStream_t>(stream), 1, p);
+  if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "rope kernel launch: %s", cudaGetErrorString(e));
+  return W4A4_OK;
+}
+
+size_t w4a4_paged_attention_workspace_bytes(const w4a4_paged_kv* cache, int T, int n_heads, int max_q_len) {
+  begin_call();
+  if (check_cache(cache) || T < 0 || n_heads < 1 || max_q_len < 0) return 0;
+  DeviceInfo* dev = nullptr;
+  if (current_device(&dev)) return 0;
+  return W4A4_ATTENTION_STATE_BYTES + (size_t)2 * dev->sm_count * pdec::Layout<128>::PART * 4;
+}
+
+int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
+                         const int32_t* cu_seqlens, const int32_t* lengths, void* out, long long out_tok_stride,
+                         long long out_head_stride, float* lse, int T, int n_heads, int max_q_len, float scale,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  begin_call();
+  int rc = check_cache(cache);
+  if (!rc) rc = check_seqs(cache, cu_seqlens, lengths, T, n_heads);
+  if (rc) return rc;
+  CHECK_ARG(max_q_len >= 0, "max_q_len must not be negative, got %d", max_q_len);
+  if (T == 0 || cache->n_seqs == 0 || max_q_len == 0) return W4A4_OK;
+  rc = check_rows("q", q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
+  if (!rc) rc = check_rows("out", out, out_tok_stride, out_head_stride, T, n_heads, cache->head_dim);
+  if (rc) return rc;
+  if (!aligned(lse, 4)) return fail(W4A4_ERR_ALIGNMENT, "lse must be 4-byte aligned");
+  DeviceInfo* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  const size_t need = w4a4_paged_attention_workspace_bytes(cache, T, n_heads, max_q_len);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(W4A4_ERR_WORKSPACE, "workspace of %zu bytes required, got %zu", need, workspace_bytes);
+  if (!aligned(workspace, 16)) return fail(W4A4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  if ((size_t)dev->sm_count > ATTN_COUNTERS) return fail(W4A4_ERR_UNSUPPORTED, "%d SMs", dev->sm_count);
+  max_q_len = max_q_len < T ? max_q_len : T;
+
+  pdec::Params p;
+  p.c = device_cache(cache);
+  p.s = device_seqs(cache, cu_seqlens, lengths, T, max_q_len);
+  p.q = q;
+  p.q_tok = q_tok_stride;
+  p.q_head = q_head_stride;
+  p.out = out;
+  p.o_tok = out_tok_stride;
+  p.o_head = out_head_stride;
+  p.lse = lse;
+  p.arrived = static_cast<int*>(workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A4_ATTENTION_STATE_BYTES);
+  p.n_heads = n_heads;
+  p.group = n_heads / cache->n_kv_heads;
+  p.box = box_slots(cache->page_size, pdec::TILE);
+  p.max_rows = 0x7fffffff;
+  p.scale_log2 = scale * kv::LOG2E;
+  CUtensorMap tk, tv;
+  rc = make_cache_map(&tk, cache, false, p.box);
+  if (!rc) rc = make_cache_map(&tv, cache, true, p.box);
+  if (rc) return rc;
+  const bool d128 = cache->head_dim == 128;
+  auto kern = d128 ? by_type(cache->dtype, pdec::paged_decode_kernel<__half, 128>, pdec::paged_decode_kernel<__nv_bfloat16, 128>)
+                   : by_type(cache->dtype, pdec::paged_decode_kernel<__half, 64>, pdec::paged_decode_kernel<__nv_bfloat16, 64>);
+  cudaError_t e = launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(pdec::THREADS), d128 ? pdec::smem_bytes<128>() : pdec::smem_bytes<64>(),
+                            static_cast<cudaStream_t>(stream), 1, tk, tv, p, (uint32_t)0);
+  if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "decode attention kernel launch: %s", cudaGetErrorString(e));
+  return W4A4_OK;
+}
+
+int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
+                           const int32_t* cu_seqlens, const int32_t* lengths, const float* lse, float* sums,
+                           long long sums_seq_stride, long long sums_head_stride, int T, int n_heads, int max_q_len,
+                           float scale, void* stream) {
+  begin_call();
+  int rc = check_cache(cache);
+  if (!rc) rc = check_seqs(cache, cu_seqlens, lengths, T, n_heads);
+  if (rc) return rc;
+  CHECK_ARG(max_q_len >= 0, "max_q_len must not be negative, got %d", max_q_len);
+  const int group = n_heads / cache->n_kv_heads;
+  if (group > csum::MAX_COLS) return fail(W4A4_ERR_UNSUPPORTED, "%d heads share a key/value head; at most %d", group, csum::MAX_COLS);
+  const long long slots = (long long)cache->max_pages * cache->page_size;
+  CHECK_ARG((sums_head_stride >= slots || cache->n_kv_heads == 1) && (sums_seq_stride >= slots || cache->n_seqs <= 1),
+            "sums strides (%lld, %lld) are below the %lld slots of a row", sums_seq_stride, sums_head_stride, slots);
+  if (T == 0 || cache->n_seqs == 0 || max_q_len == 0) return W4A4_OK;
+  rc = check_rows("q", q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
+  if (rc) return rc;
+  CHECK_ARG(lse && sums, "lse or sums is NULL");
+  if (!aligned(lse, 4) || !aligned(sums, 4)) return fail(W4A4_ERR_ALIGNMENT, "lse and sums must be 4-byte aligned");
+  DeviceInfo* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  max_q_len = max_q_len < T ? max_q_len : T;
+  csum::Params p;
+  p.c = device_cache(cache);
+  p.s = device_seqs(cache, cu_seqlens, lengths, T, max_q_len);
+  p.lse = lse;
+  p.sums = sums;
+  p.sums_seq = sums_seq_stride;
+  p.sums_head = sums_head_stride;
+  p.n_heads = n_heads;
+  p.group = group;
+  p.box = box_slots(cache->page_size, csum::TILE);
+  // the narrowest product that takes all rows of the longest sequence, 128 at most
+  const long long rows = (long long)max_q_len * group;
+  p.cols = rows >= csum::MAX_COLS ? csum::MAX_COLS : (int)((rows + 15) / 16 * 16);
+  p.toks = p.cols / group;
+  p.scale_log2 = scale * kv::LOG2E;
+  CUtensorMap tk, tq;
+  rc = make_cache_map(&tk, cache, false, p.box);
+  if (!rc) rc = make_query_map(&tq, q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim, cache->dtype, group, p.toks);
+  if (rc) return rc;
+  const bool d128 = cache->head_dim == 128;
+  auto kern = d128 ? by_type(cache->dtype, csum::cache_sums_kernel<__half, 128>, csum::cache_sums_kernel<__nv_bfloat16, 128>)
+                   : by_type(cache->dtype, csum::cache_sums_kernel<__half, 64>, csum::cache_sums_kernel<__nv_bfloat16, 64>);
+  cudaError_t e = launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(csum::THREADS), d128 ? csum::smem_bytes<128>() : csum::smem_bytes<64>(),
+                            static_cast<cudaStream_t>(stream), 1, tk, tq, p);
+  if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "weight sums kernel launch: %s", cudaGetErrorString(e));
+  return W4A4_OK;
+}
+
+int w4a4_cache_evict(const w4a4_paged_kv* cache, const w4a4_paged_kv* into, const int32_t* lengths, const float* sums,
+                     long long sums_seq_stride, long long sums_head_stride, int budget, int n_sink, int n_recent,
+                     int32_t* kept, int32_t* new_lengths, float* new_sums, void* stream) {
+  begin_call();
+  int rc = check_cache(cache);
+  if (!rc) rc = check_cache(into);
+  if (rc) return rc;
+  CHECK_ARG(into->n_seqs == cache->n_seqs && into->n_kv_heads == cache->n_kv_heads && into->head_dim == cache->head_dim &&
+                into->dtype == cache->dtype, "the caches differ in sequences, heads, head_dim or dtype");
+  CHECK_ARG(n_sink >= 0 && n_recent >= 0 && (long long)n_sink + n_recent <= budget, "n_sink (%d) and n_recent (%d) must not be negative and fit budget (%d)",
+            n_sink, n_recent, budget);
+  CHECK_ARG(budget >= 1 && budget <= (long long)into->max_pages * into->page_size, "budget (%d) must be 1 .. %lld, the slots of a sequence",
+            budget, (long long)into->max_pages * into->page_size);
+  const long long slots = (long long)cache->max_pages * cache->page_size;
+  CHECK_ARG((sums_head_stride >= slots || cache->n_kv_heads == 1) && (sums_seq_stride >= slots || cache->n_seqs <= 1),
+            "sums strides (%lld, %lld) are below the %lld slots of a row", sums_seq_stride, sums_head_stride, slots);
+  if (cache->n_seqs == 0) return W4A4_OK;
+  CHECK_ARG(lengths && sums && kept && new_lengths && new_sums, "NULL tensor pointer");
+  if (!aligned(lengths, 4) || !aligned(sums, 4) || !aligned(kept, 4) || !aligned(new_lengths, 4) || !aligned(new_sums, 4))
+    return fail(W4A4_ERR_ALIGNMENT, "lengths, sums and the outputs must be 4-byte aligned");
+  DeviceInfo* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  const long long units = (long long)cache->n_seqs * cache->n_kv_heads;
+  if (units > (1 << 24)) return fail(W4A4_ERR_UNSUPPORTED, "%lld sequences x heads", units);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  evict::SelectParams s;
+  s.lengths = lengths;
+  s.sums = sums;
+  s.sums_seq = sums_seq_stride;
+  s.sums_head = sums_head_stride;
+  s.kept = kept;
+  s.new_lengths = new_lengths;
+  s.new_sums = new_sums;
+  s.n_kv = cache->n_kv_heads;
+  s.max_slots = (int)slots;
+  s.new_slots = into->max_pages * into->page_size;
+  s.budget = budget;
+  s.sink = n_sink;
+  s.recent = n_recent;
+  cudaError_t e = launch_ex(evict::evict_select_kernel, dim3((unsigned)units), dim3(evict::SELECT_THREADS), 0, st, 1, s);
+  if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "eviction selection kernel launch: %s", cudaGetErrorString(e));
+  evict::MoveParams m;
+  m.from = device_cache(cache);
+  m.to = device_cache(into);
+  m.kept = kept;
+  m.new_lengths = new_lengths;
+  m.budget = budget;
+  // Caches that share memory: slot j may be the same place in both, so rows go in order and one block takes them all.
+  auto span = [](const w4a4_paged_kv* c, bool v) {
+    const long long* t = v ? c->v_strides : c->k_strides;
+    return (size_t)2 * ((c->n_pages - 1) * t[0] + (c->n_kv_heads - 1) * t[1] + (c->page_size - 1) * t[2] + c->head_dim);
+  };
+  auto overlap = [&](const w4a4_paged_kv* a, bool av, const w4a4_paged_kv* b, bool bv) {
+    const char* x = static_cast<const char*>(av ? a->v_pages : a->k_pages);
+    const char* y = static_cast<const char*>(bv ? b->v_pages : b->k_pages);
+    return x < y + span(b, bv) && y < x + span(a, av);
+  };
+  const bool shared = overlap(cache, false, into, false) || overlap(cache, true, into, true) || overlap(cache, false, into, true) ||
+                      overlap(cache, true, into, false);
+  m.in_place = cache->k_pages == into->k_pages && cache->v_pages == into->v_pages && cache->block_table == into->block_table &&
+               cache->table_stride == into->table_stride && cache->page_size == into->page_size &&
+               !memcmp(cache->k_strides, into->k_strides, sizeof cache->k_strides) &&
+               !memcmp(cache->v_strides, into->v_strides, sizeof cache->v_strides);
+  m.chunks = 8;
+  m.parts = 1;
+  m.rows_per_part = budget;
+  if (!shared) {
+    m.rows_per_part = 2 * evict::MOVE_UNROLL * evict::MOVE_THREADS / m.chunks;
+    m.parts = (budget + m.rows_per_part - 1) / m.rows_per_part;
+  }
+  const long long blocks = units * (2 * cache->head_dim / 8 / m.chunks) * m.parts;
+  if (blocks > 2147483647LL) return fail(W4A4_ERR_UNSUPPORTED, "%lld blocks", blocks);
+  e = launch_ex(evict::evict_move_kernel, dim3((unsigned)blocks), dim3(evict::MOVE_THREADS), 0, st, 1, m);
+  if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "eviction move kernel launch: %s", cudaGetErrorString(e));
+  return W4A4_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,162 @@
+// Norms of queries and keys, position rotation and cache write, one launch behind the qkv linear.
+//
+//   x = head row of qkv;  n = x * w / sqrt(mean(x^2) + eps)  (queries and keys, each where a weight is given);
+//   (a, b) -> (a c - b s, b c + a s)  for the pairs of the first `rot` elements, c and s of the token's position:
+//   neighbours (interleaved) or i and i + rot / 2.  Values go to the cache as they are.
+//
+// Everything between the load and the one rounding of the result is fp32.  The sum of squares is over at most 128
+// elements: 8 per lane in order, then a butterfly over the row's lanes.
+//
+// What bounds it: memory traffic for prompts, the chain offsets -> length -> page number and angles -> store for
+// decode steps.  A block takes one token, eight lanes (dim 64) or sixteen (128) a head row with one 16-byte load each,
+// so that the loads of all its rows are issued before the chain is walked; the chain's first step is one round of
+// loads whatever the number of sequences up to 32 (each lane compares one offset).
+#pragma once
+
+#include "paged_kv.cuh"
+
+namespace w4a4 {
+namespace kv {
+
+constexpr int ROPE_THREADS = 256;
+
+struct RopeParams {
+  Cache c;
+  Seqs s;
+  const void* qkv;
+  long long ld_qkv;
+  void* q_out;
+  long long q_tok, q_head;
+  const float* cos;
+  const float* sin;
+  const void* q_norm;
+  const void* k_norm;
+  const int32_t* offsets;     // per sequence: position minus slot, or NULL
+  int n_heads, rot, max_pos, interleaved;
+  float eps;
+};
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(ROPE_THREADS) qkv_rope_kernel(const RopeParams p) {
+  constexpr int LANES = DIM / 8, ROWS = ROPE_THREADS / LANES, UNROLL = 4;
+  grid_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int sub = tid % LANES;               // this thread's 8 elements of a head row
+  const int t = blockIdx.x;
+  const int n_rows = p.n_heads + 2 * p.c.n_kv;
+  const T* src = static_cast<const T*>(p.qkv) + (long long)t * p.ld_qkv + sub * 8;
+  grid_dependency_wait();
+
+  uint4 x[UNROLL];
+  auto load = [&](int row0) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int r = row0 + u * ROWS + tid / LANES;
+      if (r < n_rows) x[u] = ld_plain(reinterpret_cast<const uint4*>(src + (long long)r * DIM));
+    }
+  };
+  load(0);
+
+  // the token's sequence: how many of the n + 1 offsets are not above t, less one
+  int below = 0;
+  for (int i = lane; i <= p.s.n; i += 32) below += ld_plain(p.s.cu + i) <= t;
+  const int b = __reduce_add_sync(0xffffffffu, below) - 1;
+  if (b < 0 || b >= p.s.n) return;           // behind the last sequence: left as it is
+  const Seq q = load_seq(p.s, b);
+  const int slot = q.len - q.q_len + (t - q.q0);
+  const int pos = slot + (p.offsets ? ld_plain(p.offsets + b) : 0);
+  if (slot < 0 || (unsigned)pos >= (unsigned)p.max_pos || t >= q.q0 + q.q_len) {
+    if (tid == 0) record_error(SITE_KV_POS, b);
+    return;
+  }
+  const int page = page_of(p.c, b, slot / p.c.page), in_page = slot % p.c.page;
+
+  // cosines and sines of this thread's elements: four pairs of neighbours, or eight elements of one half
+  const int half = p.rot / 2;
+  const bool rotated = sub * 8 < p.rot;
+  const int partner = p.interleaved ? 0 : (sub * 8 < half ? half / 8 : -(half / 8));
+  const int sub0 = p.interleaved ? sub * 4 : (sub * 8 < half ? sub * 8 : sub * 8 - half);
+  float cs[8] = {}, sn[8] = {};
+  if (rotated) {
+    const float* cp = p.cos + (long long)pos * half + sub0;
+    const float* sp = p.sin + (long long)pos * half + sub0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      if (i == 0 || !p.interleaved) {
+        const float4 c4 = ld_plain(reinterpret_cast<const float4*>(cp + i)), s4 = ld_plain(reinterpret_cast<const float4*>(sp + i));
+        cs[i] = c4.x; cs[i + 1] = c4.y; cs[i + 2] = c4.z; cs[i + 3] = c4.w;
+        sn[i] = s4.x; sn[i + 1] = s4.y; sn[i + 2] = s4.z; sn[i + 3] = s4.w;
+      }
+    }
+  }
+
+  for (int row0 = 0; row0 < n_rows; row0 += UNROLL * ROWS) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int r = row0 + u * ROWS + tid / LANES;
+      const bool live = r < n_rows, is_v = r >= p.n_heads + p.c.n_kv, is_q = r < p.n_heads;
+      uint4 y = live ? x[u] : make_uint4(0, 0, 0, 0);
+      float f[8];
+      {
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = unpack2<T>(w[i]);
+          f[2 * i] = v.x;
+          f[2 * i + 1] = v.y;
+        }
+      }
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const void* nw = is_q ? p.q_norm : p.k_norm;
+      if (live && !is_v && nw != nullptr) {
+        const float r_rms = 1.f / sqrtf(ss * (1.f / DIM) + p.eps);
+        const uint4 w4 = ld_plain(reinterpret_cast<const uint4*>(static_cast<const T*>(nw) + sub * 8));
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = unpack2<T>(w[i]);
+          f[2 * i] *= r_rms * v.x;
+          f[2 * i + 1] *= r_rms * v.y;
+        }
+      }
+      float g[8];
+      if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          g[2 * i] = f[2 * i] * cs[i] - f[2 * i + 1] * sn[i];
+          g[2 * i + 1] = f[2 * i + 1] * cs[i] + f[2 * i] * sn[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float o = __shfl_sync(0xffffffffu, f[i], (lane & ~(LANES - 1)) | ((sub + partner) & (LANES - 1)));
+          g[i] = f[i] * cs[i] + (partner > 0 ? -o : o) * sn[i];
+        }
+      }
+      if (!is_v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = rotated ? g[i] : f[i];
+        y = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+      }
+      if (live) {
+        T* dst = nullptr;
+        if (is_q) {
+          dst = static_cast<T*>(p.q_out) + (long long)t * p.q_tok + (long long)r * p.q_head;
+        } else if (page >= 0) {
+          const int h = is_v ? r - p.n_heads - p.c.n_kv : r - p.n_heads;
+          dst = is_v ? static_cast<T*>(p.c.v) + page * p.c.v_page + h * p.c.v_head + in_page * p.c.v_slot
+                     : static_cast<T*>(p.c.k) + page * p.c.k_page + h * p.c.k_head + in_page * p.c.k_slot;
+        }
+        if (dst) *reinterpret_cast<uint4*>(dst + sub * 8) = y;
+      }
+    }
+    load(row0 + UNROLL * ROWS);
+  }
+}
+
+}  // namespace kv
+}  // namespace w4a4

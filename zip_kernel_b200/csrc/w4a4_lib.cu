@@ -14,12 +14,16 @@
 
 #include "../../include/w4a4_b200.h"
 #include "act_quant.cuh"
+#include "cache_evict.cuh"
+#include "cache_sums.cuh"
 #include "common.cuh"
 #include "decode_gemm.cuh"
+#include "paged_decode.cuh"
 #include "prefill_gemm.cuh"
 #include "prefill_pair_gemm.cuh"
 #include "prefill_wide_gemm.cuh"
 #include "peer_gather.cuh"
+#include "qkv_rope.cuh"
 
 namespace {
 
@@ -93,6 +97,14 @@ cudaError_t set_kernel_attributes() {
   set(pp::prefill_pair_gemm_kernel<true, true, true>, pp::smem_bytes(true));
   set(wide::prefill_wide_gemm_kernel<false>, wide::smem_bytes());
   set(wide::prefill_wide_gemm_kernel<true>, wide::smem_bytes());
+  set(csum::cache_sums_kernel<__half, 64>, csum::smem_bytes<64>());
+  set(csum::cache_sums_kernel<__half, 128>, csum::smem_bytes<128>());
+  set(csum::cache_sums_kernel<__nv_bfloat16, 64>, csum::smem_bytes<64>());
+  set(csum::cache_sums_kernel<__nv_bfloat16, 128>, csum::smem_bytes<128>());
+  set(pdec::paged_decode_kernel<__half, 64>, pdec::smem_bytes<64>());
+  set(pdec::paged_decode_kernel<__half, 128>, pdec::smem_bytes<128>());
+  set(pdec::paged_decode_kernel<__nv_bfloat16, 64>, pdec::smem_bytes<64>());
+  set(pdec::paged_decode_kernel<__nv_bfloat16, 128>, pdec::smem_bytes<128>());
   set(act_quant_kernel<128>, QUANT_MAX_SMEM);
   set(act_quant_kernel<QUANT_THREADS>, QUANT_MAX_SMEM);
   set(act_quant_kernel<128, SRC_RMSNORM>, QUANT_MAX_SMEM);
@@ -1302,3 +1314,5 @@ int w4a4_fused_dense_sparse_noalloc(const void* W_low, const void* W_high, const
 }
 
 }  // extern "C"
+
+#include "paged_api.cuh"

@@ -20,6 +20,8 @@ import torch
 from . import _lib
 from .nvtx_shim import traced
 from .pack_utils import BCOL, BROW
+from .paged_ops import (PagedKV, cache_evict_cuda, cache_weight_sums_cuda, paged_attention_cuda,
+                        qkv_rope_cache_cuda)
 
 
 def _cd(t: torch.Tensor, dtype) -> torch.Tensor:
@@ -600,4 +602,9 @@ __all__ = [
     "silu_mul_quant_cuda",
     "perm_or_none",
     "gemm_choice",
+    "PagedKV",
+    "qkv_rope_cache_cuda",
+    "paged_attention_cuda",
+    "cache_weight_sums_cuda",
+    "cache_evict_cuda",
 ]
