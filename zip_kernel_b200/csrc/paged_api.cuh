@@ -6,6 +6,7 @@ namespace {
 
 namespace kv = w4a4::kv;
 namespace pdec = w4a4::pdec;
+namespace ppre = w4a4::ppre;
 namespace csum = w4a4::csum;
 namespace evict = w4a4::evict;
 
@@ -115,8 +116,46 @@ int make_query_map(CUtensorMap* m, const void* q, long long tok, long long head,
 template <typename F16K, typename BF16K>
 auto by_type(int dtype, F16K a, BF16K b) { return dtype == W4A4_F16 ? a : b; }
 
-// ------------------------------------------------------------------ attention workspace: counters, then parts
-constexpr size_t ATTN_COUNTERS = W4A4_ATTENTION_STATE_BYTES / 4;
+// ------------------------------------------------------------------ attention plan
+// Kernels, splits and workspace (counters, then the parts of one kernel or the other) of a call; host values only.
+struct AttnPlan {
+  bool few, many;             // the kernel for few rows, the one for many
+  int few_rows;               // a sequence with at most this many rows goes to the former
+  int toks, blocks, splits;   // tokens of a row tile, blocks over rows, and over slots, of the latter
+  size_t few_parts, many_parts, many_ml, total;
+};
+// A sequence with up to this many rows (new tokens x heads of a group) goes to the kernel for few rows: one row tile of it.
+constexpr int ATTN_FEW_ROWS = pdec::ROWS;
+
+AttnPlan attn_plan(const w4a4_paged_kv* c, int T, int n_heads, int max_q, int sm_count) {
+  AttnPlan a{};
+  const int group = n_heads / c->n_kv_heads;
+  const long long rows = (long long)max_q * group;
+  a.many = rows > ATTN_FEW_ROWS && group <= ppre::ROWS;
+  a.few = !a.many || c->n_seqs > 1;                        // one sequence: whatever its length, one kernel
+  a.few_rows = !a.many ? 0x7fffffff : a.few ? ATTN_FEW_ROWS : 0;
+  a.splits = 1;
+  if (a.many) {
+    a.toks = ppre::ROWS / group;
+    const long long by_seq = (long long)c->n_seqs * ((max_q + 2 * a.toks - 1) / (2 * a.toks));
+    const long long by_all = (long long)T / (2 * a.toks) + c->n_seqs;
+    a.blocks = (int)(by_seq < by_all ? by_seq : by_all);
+    // Too few blocks for the card: the slots are split too, into pieces of at least two tiles of the longest sequence.
+    const long long base = (long long)a.blocks * c->n_kv_heads, tiles = ((long long)c->max_pages * c->page_size + ppre::TILE - 1) / ppre::TILE;
+    long long s = sm_count / base;
+    if (s > tiles / 2) s = tiles / 2;
+    a.splits = s > 16 ? 16 : s < 1 ? 1 : (int)s;
+  }
+  size_t off = W4A4_ATTENTION_STATE_BYTES;
+  a.few_parts = off;
+  if (a.few) off += (size_t)2 * sm_count * pdec::Layout<128>::PART * 4;
+  a.many_parts = off;
+  if (a.splits > 1) off += (size_t)a.splits * T * n_heads * c->head_dim * 4;
+  a.many_ml = off;
+  if (a.splits > 1) off += round_up((size_t)a.splits * T * n_heads * 8, 256);
+  a.total = off;
+  return a;
+}
 
 }  // namespace
 
@@ -169,10 +208,10 @@ int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long l
 
 size_t w4a4_paged_attention_workspace_bytes(const w4a4_paged_kv* cache, int T, int n_heads, int max_q_len) {
   begin_call();
-  if (check_cache(cache) || T < 0 || n_heads < 1 || max_q_len < 0) return 0;
+  if (check_cache(cache) || check_seqs(cache, cache->block_table, cache->block_table, T, n_heads) || max_q_len < 0) return 0;
   DeviceInfo* dev = nullptr;
   if (current_device(&dev)) return 0;
-  return W4A4_ATTENTION_STATE_BYTES + (size_t)2 * dev->sm_count * pdec::Layout<128>::PART * 4;
+  return attn_plan(cache, T, n_heads, max_q_len < T ? max_q_len : T, dev->sm_count).total;
 }
 
 int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
@@ -184,6 +223,7 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
   if (!rc) rc = check_seqs(cache, cu_seqlens, lengths, T, n_heads);
   if (rc) return rc;
   CHECK_ARG(max_q_len >= 0, "max_q_len must not be negative, got %d", max_q_len);
+  CHECK_ARG(scale > 0.f && scale < 3e38f, "scale must be positive and finite, got %g", (double)scale);
   if (T == 0 || cache->n_seqs == 0 || max_q_len == 0) return W4A4_OK;
   rc = check_rows("q", q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
   if (!rc) rc = check_rows("out", out, out_tok_stride, out_head_stride, T, n_heads, cache->head_dim);
@@ -192,40 +232,81 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
   DeviceInfo* dev = nullptr;
   rc = current_device(&dev);
   if (rc) return rc;
-  const size_t need = w4a4_paged_attention_workspace_bytes(cache, T, n_heads, max_q_len);
-  if (workspace == nullptr || workspace_bytes < need)
-    return fail(W4A4_ERR_WORKSPACE, "workspace of %zu bytes required, got %zu", need, workspace_bytes);
-  if (!aligned(workspace, 16)) return fail(W4A4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-  if ((size_t)dev->sm_count > ATTN_COUNTERS) return fail(W4A4_ERR_UNSUPPORTED, "%d SMs", dev->sm_count);
   max_q_len = max_q_len < T ? max_q_len : T;
-
-  pdec::Params p;
-  p.c = device_cache(cache);
-  p.s = device_seqs(cache, cu_seqlens, lengths, T, max_q_len);
-  p.q = q;
-  p.q_tok = q_tok_stride;
-  p.q_head = q_head_stride;
-  p.out = out;
-  p.o_tok = out_tok_stride;
-  p.o_head = out_head_stride;
-  p.lse = lse;
-  p.arrived = static_cast<int*>(workspace);
-  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + W4A4_ATTENTION_STATE_BYTES);
-  p.n_heads = n_heads;
-  p.group = n_heads / cache->n_kv_heads;
-  p.box = box_slots(cache->page_size, pdec::TILE);
-  p.max_rows = 0x7fffffff;
-  p.scale_log2 = scale * kv::LOG2E;
-  CUtensorMap tk, tv;
-  rc = make_cache_map(&tk, cache, false, p.box);
-  if (!rc) rc = make_cache_map(&tv, cache, true, p.box);
-  if (rc) return rc;
+  const AttnPlan plan = attn_plan(cache, T, n_heads, max_q_len, dev->sm_count);
+  if (workspace == nullptr || workspace_bytes < plan.total)
+    return fail(W4A4_ERR_WORKSPACE, "workspace of %zu bytes required, got %zu", plan.total, workspace_bytes);
+  if (!aligned(workspace, 16)) return fail(W4A4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  if ((size_t)dev->sm_count * 4 > W4A4_ATTENTION_STATE_BYTES) return fail(W4A4_ERR_UNSUPPORTED, "%d SMs", dev->sm_count);
+  char* ws = static_cast<char*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool d128 = cache->head_dim == 128;
-  auto kern = d128 ? by_type(cache->dtype, pdec::paged_decode_kernel<__half, 128>, pdec::paged_decode_kernel<__nv_bfloat16, 128>)
-                   : by_type(cache->dtype, pdec::paged_decode_kernel<__half, 64>, pdec::paged_decode_kernel<__nv_bfloat16, 64>);
-  cudaError_t e = launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(pdec::THREADS), d128 ? pdec::smem_bytes<128>() : pdec::smem_bytes<64>(),
-                            static_cast<cudaStream_t>(stream), 1, tk, tv, p, (uint32_t)0);
-  if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "decode attention kernel launch: %s", cudaGetErrorString(e));
+  const int group = n_heads / cache->n_kv_heads;
+
+  if (plan.few) {
+    pdec::Params p;
+    p.c = device_cache(cache);
+    p.s = device_seqs(cache, cu_seqlens, lengths, T, max_q_len);
+    p.q = q;
+    p.q_tok = q_tok_stride;
+    p.q_head = q_head_stride;
+    p.out = out;
+    p.o_tok = out_tok_stride;
+    p.o_head = out_head_stride;
+    p.lse = lse;
+    p.arrived = reinterpret_cast<int*>(ws);
+    p.parts = reinterpret_cast<float*>(ws + plan.few_parts);
+    p.n_heads = n_heads;
+    p.group = group;
+    p.box = box_slots(cache->page_size, pdec::TILE);
+    p.max_rows = plan.few_rows;
+    p.scale_log2 = scale * kv::LOG2E;
+    CUtensorMap tk, tv;
+    rc = make_cache_map(&tk, cache, false, p.box);
+    if (!rc) rc = make_cache_map(&tv, cache, true, p.box);
+    if (rc) return rc;
+    auto kern = d128 ? by_type(cache->dtype, pdec::paged_decode_kernel<__half, 128>, pdec::paged_decode_kernel<__nv_bfloat16, 128>)
+                     : by_type(cache->dtype, pdec::paged_decode_kernel<__half, 64>, pdec::paged_decode_kernel<__nv_bfloat16, 64>);
+    cudaError_t e = launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(pdec::THREADS), d128 ? pdec::smem_bytes<128>() : pdec::smem_bytes<64>(),
+                              st, 1, tk, tv, p, (uint32_t)0);
+    if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "decode attention kernel launch: %s", cudaGetErrorString(e));
+  }
+  if (plan.many) {
+    ppre::Params p;
+    p.c = device_cache(cache);
+    p.s = device_seqs(cache, cu_seqlens, lengths, T, max_q_len);
+    p.out = out;
+    p.o_tok = out_tok_stride;
+    p.o_head = out_head_stride;
+    p.lse = lse;
+    p.parts = reinterpret_cast<float*>(ws + plan.many_parts);
+    p.parts_ml = reinterpret_cast<float*>(ws + plan.many_ml);
+    p.n_heads = n_heads;
+    p.group = group;
+    p.box = box_slots(cache->page_size, ppre::TILE);
+    p.toks = plan.toks;
+    p.min_rows = plan.few_rows;
+    p.splits = plan.splits;
+    p.scale_log2 = scale * kv::LOG2E;
+    CUtensorMap tk, tv, tq;
+    rc = make_cache_map(&tk, cache, false, p.box);
+    if (!rc) rc = make_cache_map(&tv, cache, true, p.box);
+    if (!rc) rc = make_query_map(&tq, q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim, cache->dtype, group, p.toks);
+    if (rc) return rc;
+    if (cache->n_kv_heads > 65535) return fail(W4A4_ERR_UNSUPPORTED, "%d key/value heads", cache->n_kv_heads);
+    auto kern = d128 ? by_type(cache->dtype, ppre::paged_prefill_kernel<__half, 128>, ppre::paged_prefill_kernel<__nv_bfloat16, 128>)
+                     : by_type(cache->dtype, ppre::paged_prefill_kernel<__half, 64>, ppre::paged_prefill_kernel<__nv_bfloat16, 64>);
+    cudaError_t e = launch_ex(kern, dim3((unsigned)plan.blocks, (unsigned)cache->n_kv_heads, (unsigned)plan.splits), dim3(ppre::THREADS),
+                              d128 ? ppre::smem_bytes<128>() : ppre::smem_bytes<64>(), st, 1, tk, tv, tq, p);
+    if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "prompt attention kernel launch: %s", cudaGetErrorString(e));
+    if (plan.splits > 1) {
+      auto join = d128 ? by_type(cache->dtype, ppre::paged_join_kernel<__half, 128>, ppre::paged_join_kernel<__nv_bfloat16, 128>)
+                       : by_type(cache->dtype, ppre::paged_join_kernel<__half, 64>, ppre::paged_join_kernel<__nv_bfloat16, 64>);
+      const long long rows = (long long)T * n_heads;
+      e = launch_ex(join, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, 1, p);
+      if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "attention join kernel launch: %s", cudaGetErrorString(e));
+    }
+  }
   return W4A4_OK;
 }
 
@@ -238,6 +319,7 @@ int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long 
   if (!rc) rc = check_seqs(cache, cu_seqlens, lengths, T, n_heads);
   if (rc) return rc;
   CHECK_ARG(max_q_len >= 0, "max_q_len must not be negative, got %d", max_q_len);
+  CHECK_ARG(scale > 0.f && scale < 3e38f, "scale must be positive and finite, got %g", (double)scale);
   const int group = n_heads / cache->n_kv_heads;
   if (group > csum::MAX_COLS) return fail(W4A4_ERR_UNSUPPORTED, "%d heads share a key/value head; at most %d", group, csum::MAX_COLS);
   const long long slots = (long long)cache->max_pages * cache->page_size;

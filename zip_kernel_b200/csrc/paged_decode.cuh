@@ -317,7 +317,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           const int tok = w.q.q0 + (row0 + r) / p.group, hd = w.head * p.group + (row0 + r) % p.group;
           const float inv = lt > 0.f ? 1.f / lt : 0.f;       // a row that sees nothing is zero
           *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)tok * p.o_tok + (long long)hd * p.o_head + d) = pack2<T>(acc.x * inv, acc.y * inv);
-          if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = lt > 0.f ? (mx + log2f(lt)) * LN2 : neg_inf();
+          if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = lt > 0.f ? (mx + log2f(lt)) * LN2 : lt == lt ? neg_inf() : lt;
         } else {
           *reinterpret_cast<float2*>(part + 2 * ROWS + r * DIM + d) = acc;
           if (d == 0) { part[2 * r] = mx; part[2 * r + 1] = lt; }
@@ -358,7 +358,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             const int tok = w.q.q0 + (row0 + r) / p.group, hd = w.head * p.group + (row0 + r) % p.group;
             const float inv = lt > 0.f ? 1.f / lt : 0.f;
             *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)tok * p.o_tok + (long long)hd * p.o_head + d) = pack2<T>(acc.x * inv, acc.y * inv);
-            if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = lt > 0.f ? (mx + log2f(lt)) * LN2 : neg_inf();
+            if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = lt > 0.f ? (mx + log2f(lt)) * LN2 : lt == lt ? neg_inf() : lt;
           }
         }
       }

@@ -19,6 +19,7 @@
 #include "common.cuh"
 #include "decode_gemm.cuh"
 #include "paged_decode.cuh"
+#include "paged_prefill.cuh"
 #include "prefill_gemm.cuh"
 #include "prefill_pair_gemm.cuh"
 #include "prefill_wide_gemm.cuh"
@@ -101,6 +102,10 @@ cudaError_t set_kernel_attributes() {
   set(csum::cache_sums_kernel<__half, 128>, csum::smem_bytes<128>());
   set(csum::cache_sums_kernel<__nv_bfloat16, 64>, csum::smem_bytes<64>());
   set(csum::cache_sums_kernel<__nv_bfloat16, 128>, csum::smem_bytes<128>());
+  set(ppre::paged_prefill_kernel<__half, 64>, ppre::smem_bytes<64>());
+  set(ppre::paged_prefill_kernel<__half, 128>, ppre::smem_bytes<128>());
+  set(ppre::paged_prefill_kernel<__nv_bfloat16, 64>, ppre::smem_bytes<64>());
+  set(ppre::paged_prefill_kernel<__nv_bfloat16, 128>, ppre::smem_bytes<128>());
   set(pdec::paged_decode_kernel<__half, 64>, pdec::smem_bytes<64>());
   set(pdec::paged_decode_kernel<__half, 128>, pdec::smem_bytes<128>());
   set(pdec::paged_decode_kernel<__nv_bfloat16, 64>, pdec::smem_bytes<64>());
