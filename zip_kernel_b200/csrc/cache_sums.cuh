@@ -120,29 +120,24 @@ cache_sums_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     bool k_lap = false, q_lap = false, a_lap = false;      // the ring has been walked once: its places must be free
     if (warp == WARP_COPY) {
       // ---------------------------------------------------------- copies
+      PagesAhead pages;
       while (ok) {
         const int stop = (int)min((long long)w.tiles, w.tile + (end - w.at));
         const int n_rt = (w.q.q_len + p.toks - 1) / p.toks;
         for (int t = w.tile; ok && t < stop; ++t) {
           if (k_lap) ok = __all_sync(0xffffffffu, wide::wait_suspend(&k_empty[ks], kph ^ 1, SITE_SUMS_KEMPTY));
           if (!ok) break;
-          for (int b0 = 0; b0 < TILE / p.box; b0 += 32) {
-            const int slot = t * TILE + (b0 + lane) * p.box;
-            const bool mine = b0 + lane < TILE / p.box && slot < w.q.len;
-            int page = 0;
-            if (mine) {
-              page = page_of(p.c, w.b, slot / p.c.page);
-              if (page < 0) page = p.c.n_pages;
-            }
-            const int live = __popc(__ballot_sync(0xffffffffu, mine));
-            if (lane == 0) mbar_arrive_expect_tx(&k_full[ks], live * p.box * DIM * 2);      // (at most 8 boxes of 16)
-            __syncwarp();
-            if (mine)
+          const int boxes = TILE / p.box, slot = t * TILE + lane * p.box;      // (at most 8 boxes)
+          const bool mine = lane < boxes && slot < w.q.len;
+          const int page = pages.get(p.c, w.b, w.q.len, p.box, t * boxes);
+          const int live = __popc(__ballot_sync(0xffffffffu, mine));
+          if (lane == 0) mbar_arrive_expect_tx(&k_full[ks], live * p.box * DIM * 2);
+          __syncwarp();
+          if (mine)
 #pragma unroll
-              for (int h = 0; h < L::HALVES; ++h)
-                tma_load_4d(smem_u32(sm) + ks * L::K_BYTES + h * TILE * 128 + (b0 + lane) * p.box * 128, &tm_k, h * 64,
-                            slot % p.c.page, w.head, page, &k_full[ks]);
-          }
+            for (int h = 0; h < L::HALVES; ++h)
+              tma_load_4d(smem_u32(sm) + ks * L::K_BYTES + h * TILE * 128 + lane * p.box * 128, &tm_k, h * 64,
+                          slot % p.c.page, w.head, page, &k_full[ks]);
           if (++ks == K_STAGES) { ks = 0; kph ^= 1; k_lap = true; }
           for (int r = 0; r < n_rt; ++r) {
             if (n_rt == 1 && t != w.tile) continue;        // one row tile: copied once for all tiles of the unit

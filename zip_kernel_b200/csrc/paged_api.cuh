@@ -199,9 +199,12 @@ int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long l
   p.max_pos = max_pos;
   p.interleaved = interleaved != 0;
   p.eps = eps;
+  // one token a block while blocks are few, for the latency of a decode step; then four, which pay for the chain to
+  // the page number once
+  p.toks = T > 8 * dev->sm_count ? 4 : T > 4 * dev->sm_count ? 2 : 1;
   auto kern = cache->head_dim == 128 ? by_type(cache->dtype, kv::qkv_rope_kernel<__half, 128>, kv::qkv_rope_kernel<__nv_bfloat16, 128>)
                                      : by_type(cache->dtype, kv::qkv_rope_kernel<__half, 64>, kv::qkv_rope_kernel<__nv_bfloat16, 64>);
-  cudaError_t e = launch_ex(kern, dim3((unsigned)T), dim3(kv::ROPE_THREADS), 0, static_cast<cudaStream_t>(stream), 1, p);
+  cudaError_t e = launch_ex(kern, dim3((unsigned)((T + p.toks - 1) / p.toks)), dim3(kv::ROPE_THREADS), 0, static_cast<cudaStream_t>(stream), 1, p);
   if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "rope kernel launch: %s", cudaGetErrorString(e));
   return W4A4_OK;
 }
@@ -237,7 +240,7 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
   if (workspace == nullptr || workspace_bytes < plan.total)
     return fail(W4A4_ERR_WORKSPACE, "workspace of %zu bytes required, got %zu", plan.total, workspace_bytes);
   if (!aligned(workspace, 16)) return fail(W4A4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-  if ((size_t)dev->sm_count * 4 > W4A4_ATTENTION_STATE_BYTES) return fail(W4A4_ERR_UNSUPPORTED, "%d SMs", dev->sm_count);
+  if (dev->sm_count > pdec::MAX_RUNS) return fail(W4A4_ERR_UNSUPPORTED, "%d SMs", dev->sm_count);
   char* ws = static_cast<char*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool d128 = cache->head_dim == 128;
@@ -265,8 +268,13 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
     rc = make_cache_map(&tk, cache, false, p.box);
     if (!rc) rc = make_cache_map(&tv, cache, true, p.box);
     if (rc) return rc;
-    auto kern = d128 ? by_type(cache->dtype, pdec::paged_decode_kernel<__half, 128>, pdec::paged_decode_kernel<__nv_bfloat16, 128>)
-                     : by_type(cache->dtype, pdec::paged_decode_kernel<__half, 64>, pdec::paged_decode_kernel<__nv_bfloat16, 64>);
+    // (with at most eight rows in any sequence half of the row tile's registers and arithmetic fall away)
+    auto pick = [&](auto k64h, auto k64b, auto k128h, auto k128b) { return d128 ? by_type(cache->dtype, k128h, k128b) : by_type(cache->dtype, k64h, k64b); };
+    auto kern = (long long)max_q_len * group <= 8
+                    ? pick(pdec::paged_decode_kernel<__half, 64, 1>, pdec::paged_decode_kernel<__nv_bfloat16, 64, 1>,
+                           pdec::paged_decode_kernel<__half, 128, 1>, pdec::paged_decode_kernel<__nv_bfloat16, 128, 1>)
+                    : pick(pdec::paged_decode_kernel<__half, 64, 2>, pdec::paged_decode_kernel<__nv_bfloat16, 64, 2>,
+                           pdec::paged_decode_kernel<__half, 128, 2>, pdec::paged_decode_kernel<__nv_bfloat16, 128, 2>);
     cudaError_t e = launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(pdec::THREADS), d128 ? pdec::smem_bytes<128>() : pdec::smem_bytes<64>(),
                               st, 1, tk, tv, p, (uint32_t)0);
     if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "decode attention kernel launch: %s", cudaGetErrorString(e));
@@ -426,14 +434,17 @@ int w4a4_cache_evict(const w4a4_paged_kv* cache, const w4a4_paged_kv* into, cons
                cache->table_stride == into->table_stride && cache->page_size == into->page_size &&
                !memcmp(cache->k_strides, into->k_strides, sizeof cache->k_strides) &&
                !memcmp(cache->v_strides, into->v_strides, sizeof cache->v_strides);
-  m.chunks = 8;
+  const long long slices = units * (2 * cache->head_dim / 8 / evict::MOVE_CHUNKS);
   m.parts = 1;
   m.rows_per_part = budget;
   if (!shared) {
-    m.rows_per_part = 2 * evict::MOVE_UNROLL * evict::MOVE_THREADS / m.chunks;
+    // one batch a block while that fills the card, then up to four: a block's first batch pays for three loads in a row
+    int batches = (int)(slices * budget / ((long long)evict::MOVE_ROWS * 8 * dev->sm_count));
+    batches = batches < 1 ? 1 : batches > 4 ? 4 : batches;
+    m.rows_per_part = batches * evict::MOVE_ROWS;
     m.parts = (budget + m.rows_per_part - 1) / m.rows_per_part;
   }
-  const long long blocks = units * (2 * cache->head_dim / 8 / m.chunks) * m.parts;
+  const long long blocks = slices * m.parts;
   if (blocks > 2147483647LL) return fail(W4A4_ERR_UNSUPPORTED, "%lld blocks", blocks);
   e = launch_ex(evict::evict_move_kernel, dim3((unsigned)blocks), dim3(evict::MOVE_THREADS), 0, st, 1, m);
   if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "eviction move kernel launch: %s", cudaGetErrorString(e));

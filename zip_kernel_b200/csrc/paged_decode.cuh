@@ -12,9 +12,10 @@
 // is joined by the CTA that finishes its last part (the parts' order, and so the result's bits, depend on the lengths
 // alone).
 //
-// A CTA is one warp that issues copies (TMA boxes of one page each, 128-byte swizzle, a ring of tiles) and four that
-// compute, each on 16 slots of a tile with a maximum, sum and output of its own, joined at the end of a unit: no
-// barrier between the warps inside a unit.
+// A CTA is one warp that issues copies (TMA boxes of one page each, 128-byte swizzle, a ring of tiles) and two teams of
+// four that compute on alternate tiles, each warp on 16 slots of a tile with a maximum, sum and output of its own, joined
+// at the end of a unit: no barrier between the warps inside a unit.  One team alone takes about 2000 clocks from a
+// tile's arrival to handing its place back, more than the tile takes to arrive (4.3 TB/s over 148 SMs).
 //
 // Rows of values past the sequence's last slot are set to zero in shared memory first: a stale NaN there times a
 // weight of zero would be NaN.  Scores there are replaced, not added to.  Weights enter the second product as 16-bit
@@ -30,8 +31,10 @@ namespace pdec {
 
 using namespace kv;
 
-constexpr int TILE = 64, WARPS = 4, WK = TILE / WARPS, ROWS = 16;
+constexpr int TILE = 64, WK = 16, ROWS = 16;
+constexpr int SHARE = TILE / WK, TEAMS = 2, WARPS = TEAMS * SHARE;      // warps that share a tile, teams that take turns
 constexpr int THREADS = (WARPS + 1) * 32;
+constexpr int MAX_RUNS = 256;                                // CTAs of a launch
 
 enum : int { SITE_PDEC_FULL = 35, SITE_PDEC_EMPTY, SITE_PDEC_DRAIN };
 
@@ -40,12 +43,17 @@ struct Layout {
   static constexpr int HALVES = DIM / 64;                    // 128-byte wide column blocks
   static constexpr int KV_BYTES = TILE * DIM * 2;            // one tile of keys, or of values
   static constexpr int STAGE = 2 * KV_BYTES;
-  static constexpr int STAGES = DIM == 128 ? 5 : 10;
+  static constexpr int STAGES = DIM == 128 ? 6 : 12;
+  // A place of the ring belongs to one team: a team that met a place's barrier only every second phase could take the
+  // phase before the last for the last, they have the same parity.
+  static_assert(STAGES % TEAMS == 0, "a team waits for every phase of the barriers that it waits for");
   // a part of a unit in the workspace: m and l of the rows, then their outputs
   static constexpr int PART = ROWS * (2 + DIM);
-  static constexpr int joined = STAGES * STAGE;              // float [WARPS][ROWS][DIM]
-  static constexpr int ml = joined + WARPS * ROWS * DIM * 4; // float [WARPS][ROWS][2]
-  static constexpr int bars = ml + WARPS * ROWS * 2 * 4;
+  static constexpr int joined = STAGES * STAGE;              // float [SHARE][ROWS][DIM]; weights of the parts of a unit
+  static constexpr int JOINED = MAX_RUNS * ROWS * 8;
+  static_assert(SHARE * ROWS * DIM * 4 <= JOINED, "the outputs of a team fit");
+  static constexpr int ml = joined + JOINED;                 // float [SHARE][ROWS][2]
+  static constexpr int bars = ml + SHARE * ROWS * 2 * 4;
   static constexpr int total = bars + 2 * STAGES * 8 + 16;
   static_assert(1024 + total <= 232448, "shared memory of one SM");
 };
@@ -65,23 +73,36 @@ struct Params {
   float scale_log2;
 };
 
-// Row tiles and key tiles of sequence b in this kernel: none when it has no new token or more rows than max_rows.
+// What a unit costs besides its tiles - its queries, the joining of the warps - in tiles: runs are cut as if every unit
+// had that many more.  Measured, 32 sequences of 1 to 4096 slots x 8 heads: SMs busy 49 us on average and 67 us at most
+// without.
+constexpr int PAD = 3;
+
+// Row tiles and steps (PAD and then the slot tiles) of sequence b in this kernel: none when it has no new token or more
+// rows than max_rows.
 __device__ __forceinline__ void unit_shape(const Params& p, const Seq& q, int& row_tiles, int& tiles) {
   const long long rows = (long long)q.q_len * p.group;
   const bool mine = q.q_len > 0 && rows <= p.max_rows;
   row_tiles = mine ? (int)((rows + ROWS - 1) / ROWS) : 0;
-  tiles = mine ? max(1, (q.len + TILE - 1) / TILE) : 0;
+  tiles = mine ? PAD + max(1, (q.len + TILE - 1) / TILE) : 0;
 }
 
-template <typename T>
-__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// D(16x8, f32) += A(16x16) B(16x8).  With MH == 1 rows 8 to 15 are empty: d[2] and d[3] neither live nor enter.
+#define W4A4_MMA16(TYPE)                                                                                                      \
+  if constexpr (MH == 2)                                                                                                      \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"   \
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));     \
+  else {                                                                                                                      \
+    float x, y;                                                                                                               \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"   \
+        : "+f"(d[0]), "+f"(d[1]), "=f"(x), "=f"(y) : "r"(a[0]), "r"(0), "r"(a[2]), "r"(b0), "r"(b1), "f"(0.f));               \
+  }
+template <typename T, int MH>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[2 * MH], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value) { W4A4_MMA16("f16") }
+  else { W4A4_MMA16("bf16") }
 }
+#undef W4A4_MMA16
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
@@ -90,7 +111,8 @@ __device__ __forceinline__ void ldmatrix_x4_t(uint32_t (&r)[4], uint32_t a) {
 }
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
 
-template <typename T, int DIM>
+// MH: eight-row halves of a row tile that are in use
+template <typename T, int DIM, int MH>
 __global__ void __launch_bounds__(THREADS, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p,
                     const uint32_t zero) {
@@ -105,7 +127,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   if (tid == 0) {
     for (int i = 0; i < L::STAGES; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], WARPS);
+      mbar_init(&empty[i], SHARE);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
@@ -126,22 +148,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     // ------------------------------------------------------------ copies
     Walk<Params> w;
     w.start(p, begin);
+    PagesAhead pages;
     int s = 0;
     uint32_t ph = 1;
     long long n = 0;
     while (ok) {
       const int stop = (int)min((long long)w.tiles, w.tile + (end - w.at));
-      for (int t = w.tile; t < stop; ++t, ++n) {
+      for (int t = max(w.tile - PAD, 0); t < stop - PAD; ++t, ++n) {
         if (n >= L::STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph, SITE_PDEC_EMPTY));
         if (!ok) break;
         // one lane per box; boxes with no slot in use are not copied
         const int boxes = TILE / p.box, slot = t * TILE + lane * p.box;
         const bool mine = lane < boxes && slot < w.q.len;
-        int page = 0;
-        if (mine) {
-          page = page_of(p.c, w.b, slot / p.c.page);
-          if (page < 0) page = p.c.n_pages;                  // past the end of the map: reads zeros
-        }
+        const int page = pages.get(p.c, w.b, w.q.len, p.box, t * boxes);
         const int live = __popc(__ballot_sync(0xffffffffu, mine));
         if (lane == 0) mbar_arrive_expect_tx(&full[s], live * p.box * DIM * 4);
         __syncwarp();
@@ -164,76 +183,88 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int g = lane >> 2, c2 = (lane & 3) * 2;            // fragment row (and row + 8), first of two columns
     Walk<Params> w;
     w.start(p, begin);
-    int s = 0;
-    uint32_t ph = 0;
+    const int team = warp / SHARE, share = warp % SHARE;
+    uint32_t n = 0;                                          // tiles of the run before this unit
     // addresses inside a tile: this lane's ldmatrix row and the swizzle of its 16-byte chunks
-    const int k_row = warp * WK + (lane & 7) + ((lane >> 4) << 3), k_chunk = (lane >> 3) & 1;
-    const int v_row = warp * WK + (lane & 15), v_chunk = lane >> 4;
-    while (true) {
-      const int row0 = w.row_tile * ROWS, rows = min(ROWS, w.q.q_len * p.group - row0);
-      // A fragments of the rows; rows that do not exist are zero
-      uint32_t qf[DIM / 16][4];
-      int limit[2];                                          // last slot the fragment's two rows see
+    const int k_row = share * WK + (lane & 7) + ((lane >> 4) << 3), k_chunk = (lane >> 3) & 1;
+    const int v_row = share * WK + (lane & 15), v_chunk = lane >> 4;
+    // A fragments of a unit's rows (rows that do not exist are zero), and the last slots that they see
+    uint32_t qf[DIM / 16][4];
+    int limit[MH];
+    auto load_rows = [&](const Walk<Params>& u) {
+      const int left = u.q.q_len * p.group - u.row_tile * ROWS;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = g + 8 * h, tok = (row0 + r) / p.group, hd = (row0 + r) % p.group;
-        const bool live = r < rows;
-        const T* src = static_cast<const T*>(p.q) + (long long)(w.q.q0 + (live ? tok : 0)) * p.q_tok + (long long)(w.head * p.group + (live ? hd : 0)) * p.q_head;
-        limit[h] = live ? w.q.len - w.q.q_len + tok : -1;
+        const int r = g + 8 * h, tok = (u.row_tile * ROWS + r) / p.group, hd = (u.row_tile * ROWS + r) % p.group;
+        const bool live = h < MH && r < left;
+        const T* src = static_cast<const T*>(p.q) + (long long)(u.q.q0 + (live ? tok : 0)) * p.q_tok + (long long)(u.head * p.group + (live ? hd : 0)) * p.q_head;
+        if (h < MH) limit[h < MH ? h : 0] = live ? u.q.len - u.q.q_len + tok : -1;
 #pragma unroll
         for (int k = 0; k < DIM / 16; ++k) {
           qf[k][h] = live ? ld_plain(reinterpret_cast<const uint32_t*>(src + k * 16 + c2)) : 0;
           qf[k][h + 2] = live ? ld_plain(reinterpret_cast<const uint32_t*>(src + k * 16 + 8 + c2)) : 0;
         }
       }
-      float o[DIM / 8][4], m[2] = {neg_inf(), neg_inf()}, l[2] = {0.f, 0.f};
+    };
+    load_rows(w);
+    while (true) {
+      const int row0 = w.row_tile * ROWS, rows = min(ROWS, w.q.q_len * p.group - row0);
+      float o[DIM / 8][2 * MH], m[MH], l[MH];
+#pragma unroll
+      for (int h = 0; h < MH; ++h) { m[h] = neg_inf(); l[h] = 0.f; }
 #pragma unroll
       for (int i = 0; i < DIM / 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+        for (int e = 0; e < 2 * MH; ++e) o[i][e] = 0.f;
 
-      const int first = w.tile, stop = (int)min((long long)w.tiles, w.tile + (end - w.at));
-      for (int t = first; t < stop; ++t) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], ph, SITE_PDEC_FULL));
+      const int stop_step = (int)min((long long)w.tiles, w.tile + (end - w.at));
+      const int first = max(w.tile - PAD, 0), stop = max(stop_step - PAD, 0);
+      for (int t = first + ((n ^ team) & 1); t < stop; t += TEAMS) {
+        const uint32_t place = n + (t - first), s = place % L::STAGES;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], place / L::STAGES & 1, SITE_PDEC_FULL));
         if (!ok) break;
         const uint32_t kt = ring + s * L::STAGE, vt = kt + L::KV_BYTES;
-        const int slot0 = t * TILE + warp * WK;
+        const int slot0 = t * TILE + share * WK;
         if (slot0 + WK > w.q.len) {
           // the sequence ends inside these 16 slots, or before them
           const int from = max(0, w.q.len - slot0);
           for (int i = lane; i < (WK - from) * (DIM / 8); i += 32) {
-            const int r = warp * WK + from + i / (DIM / 8), ch = i % (DIM / 8);
+            const int r = share * WK + from + i / (DIM / 8), ch = i % (DIM / 8);
             sts_v4(vt + (ch >> 3) * TILE * 128 + r * 128 + ((ch & 7) << 4), make_uint4(0, 0, 0, 0));
           }
           fence_proxy_async_smem();                          // ordered before the copy that reuses the place
           __syncwarp();
         }
-        float sc[2][4] = {};
+        float sc[2][2 * MH] = {}, sd[2][2 * MH] = {};                  // two chains of products, added at the end
         uint32_t dep = 0;
 #pragma unroll
         for (int k = 0; k < DIM / 16; ++k) {
           uint32_t b[4];
           ldmatrix_x4(b, kt + (k >> 2) * TILE * 128 + k_row * 128 + ((((k & 3) * 2 + k_chunk) ^ (k_row & 7)) << 4));
-          mma_16x8x16<T>(sc[0], qf[k], b[0], b[1]);
-          mma_16x8x16<T>(sc[1], qf[k], b[2], b[3]);
+          mma_16x8x16<T, MH>(k & 1 ? sd[0] : sc[0], qf[k], b[0], b[1]);
+          mma_16x8x16<T, MH>(k & 1 ? sd[1] : sc[1], qf[k], b[2], b[3]);
         }
-        float top[2] = {m[0], m[1]};
+        float top[MH];
+        bool grown = false;
+#pragma unroll
+        for (int h = 0; h < MH; ++h) top[h] = m[h];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 2 * MH; ++e) {
             const int slot = slot0 + i * 8 + c2 + (e & 1);
-            sc[i][e] = slot <= limit[e >> 1] ? sc[i][e] * p.scale_log2 : neg_inf();
+            sc[i][e] = slot <= limit[e >> 1] ? (sc[i][e] + sd[i][e]) * p.scale_log2 : neg_inf();
             top[e >> 1] = fmaxf(top[e >> 1], sc[i][e]);
           }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < MH; ++h) {
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+          grown |= top[h] > m[h];
         }
-        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+        if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < MH; ++h) {
             const float a = top[h] > m[h] ? ex2(m[h] - top[h]) : 1.f;      // (m still minus infinity: zero)
             m[h] = top[h];
             l[h] *= a;
@@ -241,33 +272,37 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int i = 0; i < DIM / 8; ++i) { o[i][2 * h] *= a; o[i][2 * h + 1] *= a; }
           }
         }
-        const float base[2] = {m[0] == neg_inf() ? 0.f : m[0], m[1] == neg_inf() ? 0.f : m[1]};
+#pragma unroll
+        for (int h = 0; h < MH; ++h) {
+          const float base = m[h] == neg_inf() ? 0.f : m[h];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 2 * h; e < 2 * h + 2; ++e) {
+              sc[i][e] = ex2(sc[i][e] - base);
+              l[h] += sc[i][e];
+            }
+        }
+        uint32_t pf[4] = {}, pl[4] = {};                     // (slots 0-7 | 8-15) x (rows 0-7, 8-15): the A fragment
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sc[i][e] = ex2(sc[i][e] - base[e >> 1]);
-            l[e >> 1] += sc[i][e];
+          for (int h = 0; h < MH; ++h) {
+            pf[2 * i + h] = pack2<T>(sc[i][2 * h], sc[i][2 * h + 1]);
+            if constexpr (!std::is_same<T, __half>::value) {
+              const float2 hi = unpack2<T>(pf[2 * i + h]);
+              pl[2 * i + h] = pack2<T>(sc[i][2 * h] - hi.x, sc[i][2 * h + 1] - hi.y);
+            }
           }
-        const uint32_t pf[4] = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]),
-                                pack2<T>(sc[1][0], sc[1][1]), pack2<T>(sc[1][2], sc[1][3])};
-        uint32_t pl[4];
-        if constexpr (!std::is_same<T, __half>::value) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 hi = unpack2<T>(pf[i]);
-            pl[i] = pack2<T>(sc[i >> 1][(i & 1) * 2] - hi.x, sc[i >> 1][(i & 1) * 2 + 1] - hi.y);
-          }
-        }
 #pragma unroll
         for (int d = 0; d < DIM / 16; ++d) {
           uint32_t b[4];
           ldmatrix_x4_t(b, vt + (d >> 2) * TILE * 128 + v_row * 128 + ((((d & 3) * 2 + v_chunk) ^ (v_row & 7)) << 4));
-          mma_16x8x16<T>(o[2 * d], pf, b[0], b[1]);
-          mma_16x8x16<T>(o[2 * d + 1], pf, b[2], b[3]);
+          mma_16x8x16<T, MH>(o[2 * d], pf, b[0], b[1]);
+          mma_16x8x16<T, MH>(o[2 * d + 1], pf, b[2], b[3]);
           if constexpr (!std::is_same<T, __half>::value) {
-            mma_16x8x16<T>(o[2 * d], pl, b[0], b[1]);
-            mma_16x8x16<T>(o[2 * d + 1], pl, b[2], b[3]);
+            mma_16x8x16<T, MH>(o[2 * d], pl, b[0], b[1]);
+            mma_16x8x16<T, MH>(o[2 * d + 1], pl, b[2], b[3]);
           }
           dep ^= b[0] ^ b[3];
         }
@@ -275,38 +310,71 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // the keys have, their products are inputs of what came since
         __syncwarp();
         if (lane == 0) mbar_arrive_after(&empty[s], dep, zero);
-        if (++s == L::STAGES) { s = 0; ph ^= 1; }
       }
-      // ---------------------------------------------------------- join the four warps
+      n += stop - first;
+      // the next unit's queries are under way while this one is joined
+      const Walk<Params> u = w;
+      const bool more = w.at - w.tile + stop_step < end;
+      if (more) {
+        w.next_unit(p);
+        load_rows(w);
+      }
+      if (stop > first) {
+      // ---------------------------------------------------------- join the warps
       float* joined = reinterpret_cast<float*>(sm + L::joined);
       float* ml = reinterpret_cast<float*>(sm + L::ml);
+      auto place_of = [&](int h, int i) { return reinterpret_cast<float2*>(joined + (share * ROWS + g + 8 * h) * DIM + i * 8 + c2); };
+      auto leave = [&]() {                                   // this warp's m, l and outputs
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < MH; ++h) {
+          if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (share * ROWS + g + 8 * h) * 2) = make_float2(m[h], l[h]);
+          if (g + 8 * h < rows)
+#pragma unroll
+            for (int i = 0; i < DIM / 8; ++i) *place_of(h, i) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+        }
+      };
+#pragma unroll
+      for (int h = 0; h < MH; ++h) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if ((lane & 3) == 0) {
-          ml[(warp * ROWS + g + 8 * h) * 2] = m[h];
-          ml[(warp * ROWS + g + 8 * h) * 2 + 1] = l[h];
-        }
-        if (g + 8 * h < rows) {
+      }
+      if (team == 1) leave();
+      compute_barrier();
+      if (team == 0) {
+        // takes over what the other team's warp with the same slots of a tile has
 #pragma unroll
-          for (int i = 0; i < DIM / 8; ++i)
-            *reinterpret_cast<float2*>(joined + (warp * ROWS + g + 8 * h) * DIM + i * 8 + c2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+        for (int h = 0; h < MH; ++h) {
+          const float2 other = *reinterpret_cast<const float2*>(ml + (share * ROWS + g + 8 * h) * 2);
+          const float mx = fmaxf(m[h], other.x);
+          const float a = m[h] == neg_inf() ? 0.f : ex2(m[h] - mx), d = other.x == neg_inf() ? 0.f : ex2(other.x - mx);
+          m[h] = mx;
+          l[h] = a * l[h] + d * other.y;
+          if (g + 8 * h < rows)
+#pragma unroll
+            for (int i = 0; i < DIM / 8; ++i) {
+              const float2 v = *place_of(h, i);
+              o[i][2 * h] = a * o[i][2 * h] + d * v.x;
+              o[i][2 * h + 1] = a * o[i][2 * h + 1] + d * v.y;
+            }
         }
+        __syncwarp();
+        leave();
       }
       // (after a wait that gave up the warp still goes to every barrier that the others wait at)
       compute_barrier();
-      const bool whole = first == 0 && stop == w.tiles;
-      const long long u0 = w.unit_first(), u1 = u0 + w.tiles;
+      const bool whole = first == 0 && stop == u.tiles - PAD;
+      auto w_tok = [&](int r) { return u.q.q0 + (row0 + r) / p.group; };
+      auto w_head = [&](int r) { return u.head * p.group + (row0 + r) % p.group; };
+      const long long u0 = u.unit_first() + PAD, u1 = u0 + u.tiles - PAD;
       float* part = p.parts + (2 * c + (u0 < begin ? 0 : 1)) * L::PART;
       for (int e = tid; e < rows * (DIM / 2); e += WARPS * 32) {
         const int r = e / (DIM / 2), d = (e % (DIM / 2)) * 2;
         float mx = neg_inf(), lt = 0.f;
         float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) mx = fmaxf(mx, ml[(k * ROWS + r) * 2]);
+        for (int k = 0; k < SHARE; ++k) mx = fmaxf(mx, ml[(k * ROWS + r) * 2]);
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) {
+        for (int k = 0; k < SHARE; ++k) {
           const float mk = ml[(k * ROWS + r) * 2], a = mk == neg_inf() ? 0.f : ex2(mk - mx);
           const float2 v = *reinterpret_cast<const float2*>(joined + (k * ROWS + r) * DIM + d);
           lt += a * ml[(k * ROWS + r) * 2 + 1];
@@ -314,7 +382,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           acc.y += a * v.y;
         }
         if (whole) {
-          const int tok = w.q.q0 + (row0 + r) / p.group, hd = w.head * p.group + (row0 + r) % p.group;
+          const int tok = w_tok(r), hd = w_head(r);
           const float inv = lt > 0.f ? 1.f / lt : 0.f;       // a row that sees nothing is zero
           *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)tok * p.o_tok + (long long)hd * p.o_head + d) = pack2<T>(acc.x * inv, acc.y * inv);
           if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = lt > 0.f ? (mx + log2f(lt)) * LN2 : lt == lt ? neg_inf() : lt;
@@ -337,25 +405,37 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         compute_barrier();
         if (*last_flag) {
+          // the first part is the second of its run's two (the unit begins in that run), the others their run's first
+          const int parts = (int)(c1 - c0) + 1;
+          auto part_of = [&](int k) { return p.parts + (2 * (c0 + k) + (k == 0 ? 1 : 0)) * L::PART; };
+          float2* wt = reinterpret_cast<float2*>(joined);    // [parts][rows] m and l, then weight and l
+          for (int e = tid; e < parts * rows; e += WARPS * 32) wt[e] = __ldcg(reinterpret_cast<const float2*>(part_of(e / rows)) + e % rows);
+          compute_barrier();
+          if (tid < rows) {
+            float mx = neg_inf(), lt = 0.f;
+            for (int k = 0; k < parts; ++k) mx = fmaxf(mx, wt[k * rows + tid].x);
+            for (int k = 0; k < parts; ++k) {
+              float2 v = wt[k * rows + tid];
+              v.x = v.x == neg_inf() ? 0.f : ex2(v.x - mx);
+              lt += v.x * v.y;
+              wt[k * rows + tid] = v;
+            }
+            ml[2 * tid] = mx;
+            ml[2 * tid + 1] = lt;
+          }
+          compute_barrier();
           for (int e = tid; e < rows * (DIM / 2); e += WARPS * 32) {
             const int r = e / (DIM / 2), d = (e % (DIM / 2)) * 2;
-            // the first part is the second of its run's two, unless the run starts with the unit's first tile; every
-            // later run starts inside the unit
-            float mx = neg_inf(), lt = 0.f;
             float2 acc = make_float2(0.f, 0.f);
-            for (long long k = c0; k <= c1; ++k) {
-              const float* q = p.parts + (2 * k + (k == c0 ? 1 : 0)) * L::PART;
-              mx = fmaxf(mx, __ldcg(q + 2 * r));
-            }
-            for (long long k = c0; k <= c1; ++k) {
-              const float* q = p.parts + (2 * k + (k == c0 ? 1 : 0)) * L::PART;
-              const float mk = __ldcg(q + 2 * r), a = mk == neg_inf() ? 0.f : ex2(mk - mx);
-              const float2 v = __ldcg(reinterpret_cast<const float2*>(q + 2 * ROWS + r * DIM + d));
-              lt += a * __ldcg(q + 2 * r + 1);
+#pragma unroll 8
+            for (int k = 0; k < parts; ++k) {
+              const float a = wt[k * rows + r].x;
+              const float2 v = __ldcg(reinterpret_cast<const float2*>(part_of(k) + 2 * ROWS + r * DIM + d));
               acc.x += a * v.x;
               acc.y += a * v.y;
             }
-            const int tok = w.q.q0 + (row0 + r) / p.group, hd = w.head * p.group + (row0 + r) % p.group;
+            const float mx = ml[2 * r], lt = ml[2 * r + 1];
+            const int tok = w_tok(r), hd = w_head(r);
             const float inv = lt > 0.f ? 1.f / lt : 0.f;
             *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)tok * p.o_tok + (long long)hd * p.o_head + d) = pack2<T>(acc.x * inv, acc.y * inv);
             if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = lt > 0.f ? (mx + log2f(lt)) * LN2 : lt == lt ? neg_inf() : lt;
@@ -363,8 +443,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
       }
       compute_barrier();                                     // the joining buffers are free again
-      if (u0 + stop >= end) break;
-      w.next_unit(p);
+      }
+      if (!more) break;
     }
   }
   // After a wait that gave up copies may still be in flight: the block stays for a millisecond, many times what they

@@ -131,6 +131,33 @@ __device__ __forceinline__ long long total_tiles(const Params& p) {
   return w;
 }
 
+// Page numbers of a sequence's copy boxes (`box` slots each, none crosses a page), 32 at a time in the lanes of the warp
+// that issues the copies, and the next 32 already asked for: a look-up per tile would put a load's latency, longer than a
+// tile takes to arrive, between any two tiles.
+struct PagesAhead {
+  int b = -1, base = 0, cur = 0, nxt = 0;
+
+  __device__ __forceinline__ int load(const Cache& c, int len, int box, int i) const {
+    const long long slot = (long long)i * box;
+    if (slot >= len) return -1;
+    const int page = page_of(c, b, (int)(slot / c.page));
+    return page < 0 ? c.n_pages : page;                      // past the end of the map: reads zeros
+  }
+  // Whole warp: the page of box first + lane of sequence seq, for lane < TILE / box; -1 where no slot is in use.  `first`
+  // is a multiple of TILE / box, a power of two up to 32.
+  __device__ __forceinline__ int get(const Cache& c, int seq, int len, int box, int first) {
+    const int lane = threadIdx.x & 31, want = first & ~31;
+    if (seq != b || want != base) {
+      const bool next = seq == b && want == base + 32;
+      b = seq;
+      base = want;
+      cur = next ? nxt : load(c, len, box, want + lane);
+      nxt = load(c, len, box, want + 32 + lane);
+    }
+    return __shfl_sync(0xffffffffu, cur, (first - base + lane) & 31);
+  }
+};
+
 // ---------------------------------------------------------------- 16-bit float types
 template <typename T> struct Half2Of;
 template <> struct Half2Of<__half> { typedef __half2 type; };

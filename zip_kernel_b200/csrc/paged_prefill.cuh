@@ -195,14 +195,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         int s = 0;
         uint32_t ph = 1;
         const int boxes = TILE / p.box;                    // at most 8
+        PagesAhead pages;
         for (int j = j0; ok && j < j_end; ++j) {
           const int slot = j * TILE + lane * p.box;
           const bool mine = lane < boxes && slot < q.len;
-          int page = 0;
-          if (mine) {
-            page = page_of(p.c, b, slot / p.c.page);
-            if (page < 0) page = p.c.n_pages;              // past the end of the map: reads zeros
-          }
+          const int page = pages.get(p.c, b, q.len, p.box, j * boxes);
           const int live = __popc(__ballot_sync(0xffffffffu, mine)), in_page = slot % p.c.page;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {

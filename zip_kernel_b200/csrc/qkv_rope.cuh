@@ -8,9 +8,9 @@
 // elements: 8 per lane in order, then a butterfly over the row's lanes.
 //
 // What bounds it: memory traffic for prompts, the chain offsets -> length -> page number and angles -> store for
-// decode steps.  A block takes one token, eight lanes (dim 64) or sixteen (128) a head row with one 16-byte load each,
-// so that the loads of all its rows are issued before the chain is walked; the chain's first step is one round of
-// loads whatever the number of sequences up to 32 (each lane compares one offset).
+// decode steps.  Eight lanes (dim 64) or sixteen (128) take a head row with one 16-byte load each; the loads of the
+// first rows are issued before the chain is walked, whose first step is one round of loads for up to 32 sequences
+// (each lane compares one offset).
 #pragma once
 
 #include "paged_kv.cuh"
@@ -33,16 +33,21 @@ struct RopeParams {
   const void* k_norm;
   const int32_t* offsets;     // per sequence: position minus slot, or NULL
   int n_heads, rot, max_pos, interleaved;
+  int toks;                   // tokens of a block: 1, 2 or 4
   float eps;
 };
 
+// A block takes `toks` tokens, and each of them ROPE_THREADS / LANES / toks groups of LANES lanes that go through its
+// rows in turn with the token's cosines and sines in registers.
 template <typename T, int DIM>
-__global__ void __launch_bounds__(ROPE_THREADS) qkv_rope_kernel(const RopeParams p) {
-  constexpr int LANES = DIM / 8, ROWS = ROPE_THREADS / LANES, UNROLL = 4;
+__global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopeParams p) {
+  constexpr int LANES = DIM / 8, GROUPS = ROPE_THREADS / LANES, UNROLL = 4;
   grid_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31;
   const int sub = tid % LANES;               // this thread's 8 elements of a head row
-  const int t = blockIdx.x;
+  const int per_tok = GROUPS / p.toks;       // groups that share a token
+  const int t = blockIdx.x * p.toks + tid / LANES / per_tok, row_first = tid / LANES % per_tok;
+  if (t >= p.s.T) return;                    // (a warp's lanes share a token: a token has four groups or more)
   const int n_rows = p.n_heads + 2 * p.c.n_kv;
   const T* src = static_cast<const T*>(p.qkv) + (long long)t * p.ld_qkv + sub * 8;
   grid_dependency_wait();
@@ -51,7 +56,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) qkv_rope_kernel(const RopeParams
   auto load = [&](int row0) {
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int r = row0 + u * ROWS + tid / LANES;
+      const int r = row0 + u * per_tok + row_first;
       if (r < n_rows) x[u] = ld_plain(reinterpret_cast<const uint4*>(src + (long long)r * DIM));
     }
   };
@@ -66,7 +71,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) qkv_rope_kernel(const RopeParams
   const int slot = q.len - q.q_len + (t - q.q0);
   const int pos = slot + (p.offsets ? ld_plain(p.offsets + b) : 0);
   if (slot < 0 || (unsigned)pos >= (unsigned)p.max_pos || t >= q.q0 + q.q_len) {
-    if (tid == 0) record_error(SITE_KV_POS, b);
+    if (lane == 0) record_error(SITE_KV_POS, b);
     return;
   }
   const int page = page_of(p.c, b, slot / p.c.page), in_page = slot % p.c.page;
@@ -90,57 +95,61 @@ __global__ void __launch_bounds__(ROPE_THREADS) qkv_rope_kernel(const RopeParams
     }
   }
 
-  for (int row0 = 0; row0 < n_rows; row0 += UNROLL * ROWS) {
+  for (int row0 = 0; row0 < n_rows; row0 += UNROLL * per_tok) {
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int r = row0 + u * ROWS + tid / LANES;
+      const int r = row0 + u * per_tok + row_first;
       const bool live = r < n_rows, is_v = r >= p.n_heads + p.c.n_kv, is_q = r < p.n_heads;
       uint4 y = live ? x[u] : make_uint4(0, 0, 0, 0);
-      float f[8];
-      {
-        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+      if (__any_sync(0xffffffffu, live && !is_v)) {
+        float f[8];
+        {
+          const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 v = unpack2<T>(w[i]);
-          f[2 * i] = v.x;
-          f[2 * i + 1] = v.y;
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = unpack2<T>(w[i]);
+            f[2 * i] = v.x;
+            f[2 * i + 1] = v.y;
+          }
         }
-      }
-      float ss = 0.f;
+        const void* nw = is_q ? p.q_norm : p.k_norm;
+        if (p.q_norm != nullptr || p.k_norm != nullptr) {
+          float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+          for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const void* nw = is_q ? p.q_norm : p.k_norm;
-      if (live && !is_v && nw != nullptr) {
-        const float r_rms = 1.f / sqrtf(ss * (1.f / DIM) + p.eps);
-        const uint4 w4 = ld_plain(reinterpret_cast<const uint4*>(static_cast<const T*>(nw) + sub * 8));
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+          for (int o = LANES / 2; o > 0; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (nw != nullptr) {
+            const float r_rms = 1.f / sqrtf(ss * (1.f / DIM) + p.eps);
+            const uint4 w4 = ld_plain(reinterpret_cast<const uint4*>(static_cast<const T*>(nw) + sub * 8));
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 v = unpack2<T>(w[i]);
-          f[2 * i] *= r_rms * v.x;
-          f[2 * i + 1] *= r_rms * v.y;
+            for (int i = 0; i < 4; ++i) {
+              const float2 v = unpack2<T>(w[i]);
+              f[2 * i] *= r_rms * v.x;
+              f[2 * i + 1] *= r_rms * v.y;
+            }
+          }
         }
-      }
-      float g[8];
-      if (p.interleaved) {
+        float g[8];
+        if (p.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          g[2 * i] = f[2 * i] * cs[i] - f[2 * i + 1] * sn[i];
-          g[2 * i + 1] = f[2 * i + 1] * cs[i] + f[2 * i] * sn[i];
+          for (int i = 0; i < 4; ++i) {
+            g[2 * i] = f[2 * i] * cs[i] - f[2 * i + 1] * sn[i];
+            g[2 * i + 1] = f[2 * i + 1] * cs[i] + f[2 * i] * sn[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float o = __shfl_sync(0xffffffffu, f[i], (lane & ~(LANES - 1)) | ((sub + partner) & (LANES - 1)));
+            g[i] = f[i] * cs[i] + (partner > 0 ? -o : o) * sn[i];
+          }
         }
-      } else {
+        if (!is_v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float o = __shfl_sync(0xffffffffu, f[i], (lane & ~(LANES - 1)) | ((sub + partner) & (LANES - 1)));
-          g[i] = f[i] * cs[i] + (partner > 0 ? -o : o) * sn[i];
+          for (int i = 0; i < 8; ++i) f[i] = rotated ? g[i] : f[i];
+          y = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
         }
-      }
-      if (!is_v) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = rotated ? g[i] : f[i];
-        y = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
       }
       if (live) {
         T* dst = nullptr;
@@ -154,7 +163,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) qkv_rope_kernel(const RopeParams
         if (dst) *reinterpret_cast<uint4*>(dst + sub * 8) = y;
       }
     }
-    load(row0 + UNROLL * ROWS);
+    load(row0 + UNROLL * per_tok);
   }
 }
 

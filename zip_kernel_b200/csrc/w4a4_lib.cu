@@ -106,10 +106,14 @@ cudaError_t set_kernel_attributes() {
   set(ppre::paged_prefill_kernel<__half, 128>, ppre::smem_bytes<128>());
   set(ppre::paged_prefill_kernel<__nv_bfloat16, 64>, ppre::smem_bytes<64>());
   set(ppre::paged_prefill_kernel<__nv_bfloat16, 128>, ppre::smem_bytes<128>());
-  set(pdec::paged_decode_kernel<__half, 64>, pdec::smem_bytes<64>());
-  set(pdec::paged_decode_kernel<__half, 128>, pdec::smem_bytes<128>());
-  set(pdec::paged_decode_kernel<__nv_bfloat16, 64>, pdec::smem_bytes<64>());
-  set(pdec::paged_decode_kernel<__nv_bfloat16, 128>, pdec::smem_bytes<128>());
+  set(pdec::paged_decode_kernel<__half, 64, 1>, pdec::smem_bytes<64>());
+  set(pdec::paged_decode_kernel<__half, 64, 2>, pdec::smem_bytes<64>());
+  set(pdec::paged_decode_kernel<__half, 128, 1>, pdec::smem_bytes<128>());
+  set(pdec::paged_decode_kernel<__half, 128, 2>, pdec::smem_bytes<128>());
+  set(pdec::paged_decode_kernel<__nv_bfloat16, 64, 1>, pdec::smem_bytes<64>());
+  set(pdec::paged_decode_kernel<__nv_bfloat16, 64, 2>, pdec::smem_bytes<64>());
+  set(pdec::paged_decode_kernel<__nv_bfloat16, 128, 1>, pdec::smem_bytes<128>());
+  set(pdec::paged_decode_kernel<__nv_bfloat16, 128, 2>, pdec::smem_bytes<128>());
   set(act_quant_kernel<128>, QUANT_MAX_SMEM);
   set(act_quant_kernel<QUANT_THREADS>, QUANT_MAX_SMEM);
   set(act_quant_kernel<128, SRC_RMSNORM>, QUANT_MAX_SMEM);
