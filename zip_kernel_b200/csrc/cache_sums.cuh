@@ -67,6 +67,14 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// One lane of a converged warp, the same every time.  MMAs are issued under this rather than under lane == 0: the compiler
+// then knows that one thread runs the branch and keeps descriptors in uniform registers.  Measured, scores and weights
+// x values of 128 x 128 x 128 back to back: 1025 against 1111 clocks alone, and twice that beside busy softmax warps.
+__device__ __forceinline__ bool elected() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -170,7 +178,7 @@ cache_sums_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             if (ok && a_lap) ok = __all_sync(0xffffffffu, wide::wait_suspend(&acc_empty[acc], aph ^ 1, SITE_SUMS_ACCEMPTY));
             if (!ok) break;
             pre::tc_fence_after();
-            if (lane == 0) {
+            if (elected()) {
 #pragma unroll
               for (int h = 0; h < L::HALVES; ++h) {
                 const uint64_t a = pre::smem_desc_sw128(sm + ks * L::K_BYTES + h * TILE * 128);

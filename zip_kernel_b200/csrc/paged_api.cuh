@@ -117,12 +117,12 @@ template <typename F16K, typename BF16K>
 auto by_type(int dtype, F16K a, BF16K b) { return dtype == W4A4_F16 ? a : b; }
 
 // ------------------------------------------------------------------ attention plan
-// Kernels, splits and workspace (counters, then the parts of one kernel or the other) of a call; host values only.
+// Kernels and workspace (counters, then the parts of either kernel) of a call; host values only.
 struct AttnPlan {
   bool few, many;             // the kernel for few rows, the one for many
   int few_rows;               // a sequence with at most this many rows goes to the former
-  int toks, blocks, splits;   // tokens of a row tile, blocks over rows, and over slots, of the latter
-  size_t few_parts, many_parts, many_ml, total;
+  int toks;                   // tokens of a row tile of the latter
+  size_t few_parts, many_parts, total;
 };
 // A sequence with up to this many rows (new tokens x heads of a group) goes to the kernel for few rows: one row tile of it.
 constexpr int ATTN_FEW_ROWS = pdec::ROWS;
@@ -130,29 +130,16 @@ constexpr int ATTN_FEW_ROWS = pdec::ROWS;
 AttnPlan attn_plan(const w4a4_paged_kv* c, int T, int n_heads, int max_q, int sm_count) {
   AttnPlan a{};
   const int group = n_heads / c->n_kv_heads;
-  const long long rows = (long long)max_q * group;
-  a.many = rows > ATTN_FEW_ROWS && group <= ppre::ROWS;
+  a.many = (long long)max_q * group > ATTN_FEW_ROWS && group <= ppre::ROWS;
   a.few = !a.many || c->n_seqs > 1;                        // one sequence: whatever its length, one kernel
   a.few_rows = !a.many ? 0x7fffffff : a.few ? ATTN_FEW_ROWS : 0;
-  a.splits = 1;
-  if (a.many) {
-    a.toks = ppre::ROWS / group;
-    const long long by_seq = (long long)c->n_seqs * ((max_q + 2 * a.toks - 1) / (2 * a.toks));
-    const long long by_all = (long long)T / (2 * a.toks) + c->n_seqs;
-    a.blocks = (int)(by_seq < by_all ? by_seq : by_all);
-    // Too few blocks for the card: the slots are split too, into pieces of at least two tiles of the longest sequence.
-    const long long base = (long long)a.blocks * c->n_kv_heads, tiles = ((long long)c->max_pages * c->page_size + ppre::TILE - 1) / ppre::TILE;
-    long long s = sm_count / base;
-    if (s > tiles / 2) s = tiles / 2;
-    a.splits = s > 16 ? 16 : s < 1 ? 1 : (int)s;
-  }
+  a.toks = a.many ? ppre::ROWS / group : 0;
+  // (the counters are shared: the kernels of a call run one after the other and leave them zero)
   size_t off = W4A4_ATTENTION_STATE_BYTES;
   a.few_parts = off;
-  if (a.few) off += (size_t)2 * sm_count * pdec::Layout<128>::PART * 4;
+  if (a.few) off += round_up((size_t)2 * sm_count * (c->head_dim == 128 ? pdec::Layout<128>::PART : pdec::Layout<64>::PART) * 4, 256);
   a.many_parts = off;
-  if (a.splits > 1) off += (size_t)a.splits * T * n_heads * c->head_dim * 4;
-  a.many_ml = off;
-  if (a.splits > 1) off += round_up((size_t)a.splits * T * n_heads * 8, 256);
+  if (a.many) off += (size_t)2 * sm_count * (c->head_dim == 128 ? ppre::Layout<128>::PART : ppre::Layout<64>::PART) * 4;
   a.total = off;
   return a;
 }
@@ -287,33 +274,24 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
     p.o_tok = out_tok_stride;
     p.o_head = out_head_stride;
     p.lse = lse;
+    p.arrived = reinterpret_cast<int*>(ws);
     p.parts = reinterpret_cast<float*>(ws + plan.many_parts);
-    p.parts_ml = reinterpret_cast<float*>(ws + plan.many_ml);
     p.n_heads = n_heads;
     p.group = group;
     p.box = box_slots(cache->page_size, ppre::TILE);
     p.toks = plan.toks;
     p.min_rows = plan.few_rows;
-    p.splits = plan.splits;
     p.scale_log2 = scale * kv::LOG2E;
     CUtensorMap tk, tv, tq;
     rc = make_cache_map(&tk, cache, false, p.box);
     if (!rc) rc = make_cache_map(&tv, cache, true, p.box);
     if (!rc) rc = make_query_map(&tq, q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim, cache->dtype, group, p.toks);
     if (rc) return rc;
-    if (cache->n_kv_heads > 65535) return fail(W4A4_ERR_UNSUPPORTED, "%d key/value heads", cache->n_kv_heads);
     auto kern = d128 ? by_type(cache->dtype, ppre::paged_prefill_kernel<__half, 128>, ppre::paged_prefill_kernel<__nv_bfloat16, 128>)
                      : by_type(cache->dtype, ppre::paged_prefill_kernel<__half, 64>, ppre::paged_prefill_kernel<__nv_bfloat16, 64>);
-    cudaError_t e = launch_ex(kern, dim3((unsigned)plan.blocks, (unsigned)cache->n_kv_heads, (unsigned)plan.splits), dim3(ppre::THREADS),
+    cudaError_t e = launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(ppre::THREADS),
                               d128 ? ppre::smem_bytes<128>() : ppre::smem_bytes<64>(), st, 1, tk, tv, tq, p);
     if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "prompt attention kernel launch: %s", cudaGetErrorString(e));
-    if (plan.splits > 1) {
-      auto join = d128 ? by_type(cache->dtype, ppre::paged_join_kernel<__half, 128>, ppre::paged_join_kernel<__nv_bfloat16, 128>)
-                       : by_type(cache->dtype, ppre::paged_join_kernel<__half, 64>, ppre::paged_join_kernel<__nv_bfloat16, 64>);
-      const long long rows = (long long)T * n_heads;
-      e = launch_ex(join, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, 1, p);
-      if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "attention join kernel launch: %s", cudaGetErrorString(e));
-    }
   }
   return W4A4_OK;
 }

@@ -6,8 +6,8 @@
 // rows holds whole tokens, so the heads of a group share every key and value tile, and a block has two row tiles, whose
 // products and softmax alternate: while the tensor cores work on one, the other's softmax warps have the CUDA cores.
 //
-// Roles: a warp that issues copies (TMA boxes of one page each), a thread that issues MMAs, four warps of softmax per
-// row tile.  Scores are 128 x 128 fp32 in tensor memory, thread = row; the weights go back there as 16-bit pairs over
+// Roles: a warp that plans (finds the CTA's next unit of work and writes it to shared memory), a warp that issues copies
+// (TMA boxes of one page each), a thread that issues MMAs, four warps of softmax per row tile.  Scores are 128 x 128 fp32 in tensor memory, thread = row; the weights go back there as 16-bit pairs over
 // the scores and are the A operand of the second product, whose B operand is the value tile as it lands (slots x
 // elements, read along the elements).  The output stays in tensor memory; it is multiplied by exp(m_old - m_new) only
 // when some row's maximum has grown by more than a factor of 2^8, until when the weights are simply larger than one
@@ -31,13 +31,14 @@ using csum::idesc_f16;
 using csum::umma_f16;
 
 constexpr int TILE = 128, ROWS = 128;                        // slots of a tile, rows of a row tile
-constexpr int WARP_COPY = 8, WARP_MMA = 9, THREADS = 12 * 32;
-constexpr int REG_ISSUE = 56, REG_SOFTMAX = 224;
+constexpr int WARP_COPY = 8, WARP_MMA = 9, WARP_PLAN = 10, THREADS = 12 * 32;
+constexpr int WORKS = 4;                                     // units planned ahead
+constexpr int REG_ISSUE = 72, REG_SOFTMAX = 216;
 static_assert(REG_ISSUE + 2 * REG_SOFTMAX <= 3 * 168, "the warpgroups share the registers of the launch");
 constexpr int TMEM_COLS = 512, TMEM_O = 256;
 constexpr float GROWTH = 8.f;                                // (log2) of a row's maximum before the output follows
 
-enum : int { SITE_PPRE_EMPTY = 80, SITE_PPRE_Q, SITE_PPRE_K, SITE_PPRE_V, SITE_PPRE_P, SITE_PPRE_S, SITE_PPRE_VZERO, SITE_PPRE_O };
+enum : int { SITE_PPRE_EMPTY = 80, SITE_PPRE_Q, SITE_PPRE_K, SITE_PPRE_V, SITE_PPRE_P, SITE_PPRE_S, SITE_PPRE_VZERO, SITE_PPRE_O, SITE_PPRE_QEMPTY, SITE_PPRE_OEMPTY, SITE_PPRE_WORK, SITE_PPRE_WFREE, SITE_PPRE_MEET };
 
 template <int DIM>
 struct Layout {
@@ -45,8 +46,10 @@ struct Layout {
   static constexpr int SLOT = TILE * DIM * 2;                // a tile of keys, or of values, or of query rows
   static constexpr int STAGES = DIM == 128 ? 5 : 10;
   static constexpr int q = STAGES * SLOT;
-  static constexpr int bars = q + 2 * SLOT;
-  static constexpr int total = bars + (2 * STAGES + 8) * 8 + 16;
+  static constexpr int works = q + 2 * SLOT;                 // Work [WORKS]
+  static constexpr int bars = works + WORKS * 64;
+  static constexpr int total = bars + (2 * STAGES + 13 + 2 * WORKS) * 8 + 16;
+  static constexpr int PART = 2 * ROWS * (DIM + 2);          // of a unit in the workspace: float2 m, l [row], float4 [dim / 4][row]
   static_assert(1024 + total <= 232448, "shared memory of one SM");
 };
 template <int DIM> inline size_t smem_bytes() { return 1024 + Layout<DIM>::total; }
@@ -57,16 +60,131 @@ struct Params {
   void* out;
   long long o_tok, o_head;
   float* lse;                 // (T, n_heads), or NULL
-  float* parts;               // [splits][T * n_heads][dim], or NULL when splits == 1
-  float* parts_ml;            // [splits][T * n_heads][2]
-  int n_heads, group, box, toks, min_rows, splits;
+  float* parts;               // [2 * grid][Layout::PART]
+  int* arrived;               // [grid]: finished parts of the unit that is cut first in that run; zero between calls
+  int n_heads, group, box, toks, min_rows;
   float scale_log2;
 };
 
-// Blocks (pairs of row tiles) of sequence b in this kernel.
+// A unit is a pair of row tiles of one (sequence, key/value head).  All units lie end to end, measured in slots: those that
+// a unit's last row sees and PAD more for what a unit costs besides its tiles; the row is cut into one equal run per
+// CTA.  A unit that falls into several runs is joined by the CTA that finishes its last part, in the order of the parts.
+constexpr int PAD = 192;
+constexpr int MIN_RUN = 4 * TILE;                            // shorter runs cost more in joining than they save
+
+struct Unit {
+  int b, head, blk, blocks;
+  long long past;             // slots before the sequence's new tokens, not below zero
+  long long u0, weight;       // place in the row
+  Seq q;
+};
+
+// Units of sequence b for each head in this kernel.
 __device__ __forceinline__ int seq_blocks(const Params& p, const Seq& q) {
   return (long long)q.q_len * p.group > p.min_rows ? (q.q_len + 2 * p.toks - 1) / (2 * p.toks) : 0;
 }
+// Weight of the first `blk` units of a head, all of them whole.
+__device__ __forceinline__ long long blocks_weight(const Params& p, long long past, long long blk) {
+  return blk * (PAD + past) + (long long)p.toks * blk * (blk + 1);
+}
+__device__ __forceinline__ long long head_weight(const Params& p, const Seq& q, int blocks) {
+  const long long past = max(q.len - q.q_len, 0);
+  return blocks > 0 ? blocks_weight(p, past, blocks - 1) + PAD + past + q.q_len : 0;
+}
+
+struct Units {
+  long long total, count;     // weight and number of all units (whole warp)
+  __device__ __forceinline__ void sum(const Params& p) {
+    total = count = 0;
+    for (int b = threadIdx.x & 31; b < p.s.n; b += 32) {
+      const Seq q = load_seq(p.s, b);
+      const int n = seq_blocks(p, q);
+      total += head_weight(p, q, n) * p.c.n_kv;
+      count += (long long)n * p.c.n_kv;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      count += __shfl_xor_sync(0xffffffffu, count, o);
+    }
+  }
+};
+
+__device__ __forceinline__ void unit_weight(const Params& p, Unit& u) {
+  u.weight = PAD + u.past + min((u.blk + 1) * 2 * p.toks, u.q.q_len);
+}
+// The unit at place x of the row, x below the total (whole warp).
+__device__ __forceinline__ Unit unit_at(const Params& p, long long x) {
+  const int lane = threadIdx.x & 31;
+  Unit u{};
+  long long before = 0;
+  for (int base = 0; base < p.s.n; base += 32) {
+    long long w = 0;
+    if (base + lane < p.s.n) {
+      const Seq q = load_seq(p.s, base + lane);
+      w = head_weight(p, q, seq_blocks(p, q)) * p.c.n_kv;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const long long a = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += a;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, before + w > x);
+    if (over) {
+      const int i = __ffs(over) - 1;
+      const long long w1 = __shfl_sync(0xffffffffu, w, (i - 1) & 31);
+      before += i ? w1 : 0;
+      u.b = base + i;
+      u.q = load_seq(p.s, u.b);
+      u.blocks = seq_blocks(p, u.q);
+      u.past = max(u.q.len - u.q.q_len, 0);
+      const long long per_head = head_weight(p, u.q, u.blocks);
+      u.head = (int)((x - before) / per_head);
+      const long long start = before + u.head * per_head;
+      int lo = 0, hi = u.blocks - 1;                         // the last block that does not start behind x
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (start + blocks_weight(p, u.past, mid) <= x) lo = mid;
+        else hi = mid - 1;
+      }
+      u.blk = lo;
+      u.u0 = start + blocks_weight(p, u.past, lo);
+      unit_weight(p, u);
+      return u;
+    }
+    before += __shfl_sync(0xffffffffu, w, 31);
+  }
+  return u;
+}
+// The next unit (there is one).
+__device__ __forceinline__ void next_unit(const Params& p, Unit& u) {
+  u.u0 += u.weight;
+  if (++u.blk == u.blocks) {
+    u.blk = 0;
+    if (++u.head == p.c.n_kv) {
+      u.head = 0;
+      do {
+        u.q = load_seq(p.s, ++u.b);
+        u.blocks = seq_blocks(p, u.q);
+      } while (u.blocks == 0);
+      u.past = max(u.q.len - u.q.q_len, 0);
+    }
+  }
+  unit_weight(p, u);
+}
+
+// What a run has of a unit, as the planning warp leaves it in shared memory: tiles j0 .. of it, for either row tile up to
+// n_row (none when that is j0).
+struct Work {
+  int live;                   // 0: the run has ended
+  int b, head, tok0;          // sequence, key/value head, first token (of the sequence) of the unit
+  int q0, q_len, len;
+  int j0, n_row[2];
+  int whole;                  // the unit is in this run alone
+  int part, first_run, parts; // its part in the workspace; the run of its first part, and how many there are
+  int pad[2];
+};
+static_assert(sizeof(Work) == 64, "the place of one");
 
 // descriptor of a B operand whose rows in shared memory are the K side (slots) and run along N (elements): 64 elements
 // under the 128-byte swizzle, 8 slots 1024 bytes apart, the next 64 elements `halves` bytes on
@@ -99,7 +217,33 @@ __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Bounded wait that never sleeps, for the thread that issues the MMAs: it wakes from a sleeping wait about 450 clocks after
+// the arrival, and every hand-over between products and softmax would pay that.
+__device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity, int site) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (done) return true;
+    if ((i & 0xffff) == 0) {                               // (65536 polls are some milliseconds)
+      if (t0 == 0) t0 = wide::timer_ns();
+      else if (i > wide::WAIT_POLLS && wide::timer_ns() - t0 > wide::WAIT_NS) break;
+    }
+  }
+  record_error(site, parity);
+  return false;
+}
 
 template <typename T, int DIM>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -110,21 +254,31 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::bars);    // ring of key and value tiles in turn
   uint64_t* empty = full + L::STAGES;
-  uint64_t* q_full = empty + L::STAGES;                          // [2] per row tile, as the next three
-  uint64_t* s_full = q_full + 2;
+  uint64_t* q_full = empty + L::STAGES;                          // [2] per row tile, as the next five
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* s_full = q_empty + 2;
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* o_empty = o_full + 2;
+  uint64_t* w_full = o_empty + 2;                                // [WORKS]
+  uint64_t* w_empty = w_full + WORKS;
+  uint64_t* meet = w_empty + WORKS;                              // the eight softmax warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet + 1);
+  int* last_flag = reinterpret_cast<int*>(tmem_slot + 1);
   grid_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < L::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 4);
     }
+    for (int i = 0; i < WORKS; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 10); }
+    mbar_init(meet, 8);
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -138,72 +292,102 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   if (warp == WARP_COPY) grid_dependency_wait_for_async_reads();
   else grid_dependency_wait();
 
-  // The block's sequence: the last blocks of a sequence, which see most slots, come first.
-  int b = -1, blk = 0;
-  Seq q{};
-  {
-    int before = 0;
-    const int r = blockIdx.x;
-    for (int base = 0; base < p.s.n && b < 0; base += 32) {
-      int n = base + lane < p.s.n ? seq_blocks(p, load_seq(p.s, base + lane)) : 0, w = n;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const int a = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += a;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, before + w > r);
-      if (past) {
-        const int i = __ffs(past) - 1;
-        b = base + i;
-        blk = before + __shfl_sync(0xffffffffu, w, i) - 1 - r;
-        q = load_seq(p.s, b);
-      }
-      before += __shfl_sync(0xffffffffu, w, 31);
-    }
-  }
-  const int head = blockIdx.y, split = blockIdx.z;
+  Work* works = reinterpret_cast<Work*>(sm + L::works);
   bool ok = true;                                          // no wait of this thread has given up
-  if (b >= 0) {
-    const int tok0 = blk * 2 * p.toks, past_len = q.len - q.q_len;
-    // tiles of either row tile up to its last row's slot; none when it has no row or its rows see nothing
-    int n_all[2], n[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int t0 = tok0 + t * p.toks, t1 = min(t0 + p.toks, q.q_len);
-      n_all[t] = t0 < q.q_len ? max(0, (past_len + t1 + TILE - 1) / TILE) : 0;
-    }
-    // this split's share of the tiles of the longer one
-    const int n_max = max(n_all[0], n_all[1]);
-    const int j0 = (int)((long long)n_max * split / p.splits), j1 = (int)((long long)n_max * (split + 1) / p.splits);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) n[t] = max(j0, min(j1, n_all[t]));
-    const int j_end = max(n[0], n[1]);
+  uint32_t nw = 0;                                         // units taken so far
+  // The next unit of work (whole warp), nullptr after the last; handed back with work_done.
+  auto next_work = [&]() -> const Work* {
+    if (ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(&w_full[nw % WORKS], nw / WORKS & 1, SITE_PPRE_WORK));
+    return ok && works[nw % WORKS].live ? &works[nw % WORKS] : nullptr;
+  };
+  auto work_done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&w_empty[nw % WORKS]);
+    ++nw;
+  };
 
-    if (warp >= WARP_COPY) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_ISSUE));
-      if (warp == WARP_COPY) {
-        // ---------------------------------------------------------- copies
+  if (warp >= WARP_COPY) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_ISSUE));
+    if (warp == WARP_PLAN) {
+      // ---------------------------------------------------------- planning
+      Units all;
+      all.sum(p);
+      const long long runs = min((long long)gridDim.x, max(all.count, all.total / MIN_RUN)), run = blockIdx.x;
+      auto put = [&](const Work& w) {
+        if (nw >= WORKS) ok = __all_sync(0xffffffffu, wide::wait_suspend(&w_empty[nw % WORKS], (nw / WORKS - 1) & 1, SITE_PPRE_WFREE));
+        if (!ok) return;
         if (lane == 0) {
-          for (int t = 0; t < 2; ++t) {
-            if (n[t] == j0) continue;
-            mbar_arrive_expect_tx(&q_full[t], p.toks * p.group * DIM * 2);
-            for (int h = 0; h < L::HALVES; ++h)
-              tma_load_3d(sm + L::q + t * L::SLOT + h * ROWS * 128, &tm_q, h * 64, head * p.group, q.q0 + tok0 + t * p.toks, &q_full[t]);
-          }
+          works[nw % WORKS] = w;
+          mbar_arrive(&w_full[nw % WORKS]);                // (releases the writes before it)
         }
         __syncwarp();
-        int s = 0;
-        uint32_t ph = 1;
-        const int boxes = TILE / p.box;                    // at most 8
-        PagesAhead pages;
+        ++nw;
+      };
+      if (run < runs) {
+        const long long begin = run * all.total / runs, end = (run + 1) * all.total / runs;
+        Unit u = unit_at(p, begin);
+        while (ok) {
+          Work w{};
+          w.live = 1;
+          w.b = u.b;
+          w.head = u.head;
+          w.q0 = u.q.q0;
+          w.q_len = u.q.q_len;
+          w.len = u.q.len;
+          w.tok0 = u.blk * 2 * p.toks;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int t0 = w.tok0 + t * p.toks, t1 = min(t0 + p.toks, w.q_len);
+            w.n_row[t] = t0 < w.q_len ? max(0, (w.len - w.q_len + t1 + TILE - 1) / TILE) : 0;
+          }
+          const int n = max(1, max(w.n_row[0], w.n_row[1]));       // (a unit that sees nothing still has zeros to write)
+          const long long first = u.u0 + PAD;              // where the unit's first tile lies in the row
+          const int j1 = (int)min((max(end - first, 0LL) + TILE - 1) / TILE, (long long)n);
+          w.j0 = (int)min((max(begin - first, 0LL) + TILE - 1) / TILE, (long long)n);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) w.n_row[t] = max(w.j0, min(j1, w.n_row[t]));
+          w.whole = w.j0 == 0 && j1 == n;
+          // runs the unit falls into: run(x) = the c with c * total / runs <= x < (c + 1) * total / runs
+          w.first_run = (int)(((first + 1) * runs - 1) / all.total);
+          w.parts = (int)(((first + (long long)(n - 1) * TILE + 1) * runs - 1) / all.total) - w.first_run + 1;
+          w.part = (int)(2 * run) + (first < begin ? 0 : 1);
+          if (j1 > w.j0) put(w);
+          if (u.u0 + u.weight >= end) break;
+          next_unit(p, u);
+        }
+      }
+      if (ok) put(Work{});
+    } else if (warp == WARP_COPY) {
+      // ---------------------------------------------------------- copies
+      int s = 0;
+      uint32_t ph = 1, uses[2] = {0, 0};
+      bool lap = false;
+      const int boxes = TILE / p.box;                      // at most 8
+      PagesAhead pages;
+      while (const Work* w = next_work()) {
+        const int b = w->b, head = w->head, len = w->len, j0 = w->j0, n_row[2] = {w->n_row[0], w->n_row[1]}, tok = w->q0 + w->tok0;
+        work_done();
+        for (int t = 0; ok && t < 2; ++t) {
+          if (n_row[t] == j0) continue;
+          if (uses[t] > 0) ok = __all_sync(0xffffffffu, wide::wait_suspend(&q_empty[t], (uses[t] - 1) & 1, SITE_PPRE_QEMPTY));
+          if (!ok) break;
+          ++uses[t];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full[t], p.toks * p.group * DIM * 2);
+            for (int h = 0; h < L::HALVES; ++h)
+              tma_load_3d(sm + L::q + t * L::SLOT + h * ROWS * 128, &tm_q, h * 64, head * p.group, tok + t * p.toks, &q_full[t]);
+          }
+          __syncwarp();
+        }
+        const int j_end = max(n_row[0], n_row[1]);
         for (int j = j0; ok && j < j_end; ++j) {
           const int slot = j * TILE + lane * p.box;
-          const bool mine = lane < boxes && slot < q.len;
-          const int page = pages.get(p.c, b, q.len, p.box, j * boxes);
+          const bool mine = lane < boxes && slot < len;
+          const int page = pages.get(p.c, b, len, p.box, j * boxes);
           const int live = __popc(__ballot_sync(0xffffffffu, mine)), in_page = slot % p.c.page;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            if (2 * (j - j0) + kv >= L::STAGES && ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(&empty[s], ph, SITE_PPRE_EMPTY));
+            if (lap && ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(&empty[s], ph, SITE_PPRE_EMPTY));
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(&full[s], live * p.box * DIM * 2);
             __syncwarp();
@@ -212,70 +396,75 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
               for (int h = 0; h < L::HALVES; ++h)
                 tma_load_4d(smem_u32(sm) + s * L::SLOT + h * TILE * 128 + lane * p.box * 128, kv ? &tm_v : &tm_k, h * 64, in_page,
                             head, page, &full[s]);
-            if (++s == L::STAGES) { s = 0; ph ^= 1; }
+            if (++s == L::STAGES) { s = 0; ph ^= 1; lap = true; }
           }
         }
-      } else if (warp == WARP_MMA) {
-        // ---------------------------------------------------------- MMAs
-        const uint32_t id_s = idesc_f16<T>(TILE), id_o = idesc_f16<T>(DIM) | (1u << 16);
-        int s = 0;
-        uint32_t ph = 0;
-        auto next = [&]() { if (++s == L::STAGES) { s = 0; ph ^= 1; } };
-        auto scores = [&](int t, int slot) {
-          if (lane == 0) {
+      }
+    } else if (warp == WARP_MMA && csum::elected()) {
+      // ---------------------------------------------------------- MMAs: one thread
+      const uint32_t id_s = idesc_f16<T>(TILE), id_o = idesc_f16<T>(DIM) | (1u << 16);
+      int s = 0;
+      uint32_t ph = 0, uses[2] = {0, 0}, steps[2] = {0, 0};
+      auto next = [&]() { if (++s == L::STAGES) { s = 0; ph ^= 1; } };
+      auto scores = [&](int t, int slot, bool last) {
 #pragma unroll
-            for (int h = 0; h < L::HALVES; ++h) {
-              const uint64_t a = pre::smem_desc_sw128(sm + L::q + t * L::SLOT + h * ROWS * 128);
-              const uint64_t bd = pre::smem_desc_sw128(sm + slot * L::SLOT + h * TILE * 128);
+        for (int h = 0; h < L::HALVES; ++h) {
+          const uint64_t a = pre::smem_desc_sw128(sm + L::q + t * L::SLOT + h * ROWS * 128);
+          const uint64_t bd = pre::smem_desc_sw128(sm + slot * L::SLOT + h * TILE * 128);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16(tmem_base + t * TILE, a + 2 * k, bd + 2 * k, h > 0 || k > 0, id_s);
-            }
-            pre::umma_commit(&s_full[t]);
-          }
-          __syncwarp();
-        };
-        auto release = [&](int slot) {
-          if (lane == 0) pre::umma_commit(&empty[slot]);
-          __syncwarp();
-        };
+          for (int k = 0; k < 4; ++k) umma_f16(tmem_base + t * TILE, a + 2 * k, bd + 2 * k, h > 0 || k > 0, id_s);
+        }
+        pre::umma_commit(&s_full[t]);
+        if (last) pre::umma_commit(&q_empty[t]);
+      };
+      auto release = [&](int slot) { pre::umma_commit(&empty[slot]); };
+      while (ok) {
+        ok = wide::wait_suspend(&w_full[nw % WORKS], nw / WORKS & 1, SITE_PPRE_WORK);
+        const Work* w = &works[nw % WORKS];
+        if (!ok || !w->live) break;
+        const int j0 = w->j0, n_row[2] = {w->n_row[0], w->n_row[1]};
+        mbar_arrive(&w_empty[nw++ % WORKS]);
+        const int j_end = max(n_row[0], n_row[1]);
         if (j0 < j_end) {
-          ok = __all_sync(0xffffffffu, wide::wait_suspend(&full[s], ph, SITE_PPRE_K));
+          ok = wait_spin(&full[s], ph, SITE_PPRE_K);
           for (int t = 0; ok && t < 2; ++t) {
-            if (n[t] == j0) continue;
-            ok = __all_sync(0xffffffffu, wide::wait_suspend(&q_full[t], 0, SITE_PPRE_Q));
+            if (n_row[t] == j0) continue;
+            ok = wait_spin(&q_full[t], uses[t] & 1, SITE_PPRE_Q);
             if (!ok) break;
             pre::tc_fence_after();
-            scores(t, s);
+            scores(t, s, j0 + 1 == n_row[t]);
           }
           if (ok) release(s);
           next();
         }
         for (int j = j0; ok && j < j_end; ++j) {
           const int vs = s;
-          ok = __all_sync(0xffffffffu, wide::wait_suspend(&full[s], ph, SITE_PPRE_V));
+          ok = wait_spin(&full[s], ph, SITE_PPRE_V);
           next();
           const int ks = s;
           const uint32_t kph = ph;
           bool k_here = false;
           for (int t = 0; ok && t < 2; ++t) {
-            if (j >= n[t]) continue;
-            ok = __all_sync(0xffffffffu, wide::wait_suspend(&p_full[t], (j - j0) & 1, SITE_PPRE_P));
+            if (j >= n_row[t]) continue;
+            ok = wait_spin(&p_full[t], steps[t] & 1, SITE_PPRE_P);
+            ++steps[t];
+            if (ok && j == j0) {                           // the output of the unit before has been read
+              if (uses[t] > 0) ok = wide::wait_suspend(&o_empty[t], (uses[t] - 1) & 1, SITE_PPRE_OEMPTY);
+              ++uses[t];
+            }
             if (!ok) break;
             pre::tc_fence_after();
-            if (lane == 0) {
-              const uint64_t bd = smem_desc_mn_sw128(smem_u32(sm + vs * L::SLOT), TILE * 128);
+            const uint64_t bd = smem_desc_mn_sw128(smem_u32(sm + vs * L::SLOT), TILE * 128);
 #pragma unroll
-              for (int k = 0; k < TILE / 16; ++k)
-                umma_f16_ta(tmem_base + TMEM_O + t * DIM, tmem_base + t * TILE + k * 8, bd + k * (2048 >> 4), j > j0 || k > 0, id_o);
-              if (j == n[t] - 1) pre::umma_commit(&o_full[t]);
-            }
-            __syncwarp();
-            if (j + 1 < n[t]) {
-              if (!k_here) ok = __all_sync(0xffffffffu, wide::wait_suspend(&full[ks], kph, SITE_PPRE_K));
+            for (int k = 0; k < TILE / 16; ++k)
+              umma_f16_ta(tmem_base + TMEM_O + t * DIM, tmem_base + t * TILE + k * 8, bd + k * (2048 >> 4), j > j0 || k > 0, id_o);
+            if (j == n_row[t] - 1) pre::umma_commit(&o_full[t]);
+            if (j + 1 < n_row[t]) {
+              if (!k_here) ok = wait_spin(&full[ks], kph, SITE_PPRE_K);
               k_here = true;
               if (!ok) break;
               pre::tc_fence_after();
-              scores(t, ks);
+              scores(t, ks, j + 2 == n_row[t]);
             }
           }
           if (ok) release(vs);
@@ -285,127 +474,192 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           }
         }
       }
-    } else {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFTMAX));
-      // ------------------------------------------------------------ softmax: thread = row
-      const int t = warp >> 2, row = tid & 127;
-      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t ts = tmem_base + lanes + t * TILE, to = tmem_base + lanes + TMEM_O + t * DIM;
-      const int tok = tok0 + t * p.toks + row / p.group;
-      const bool live = row < p.toks * p.group && tok < q.q_len;
-      const int limit = live ? past_len + tok : -1;        // last slot this row sees
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFTMAX));
+    // -------------------------------------------------------------- softmax: thread = row
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem_base + lanes + t * TILE, to = tmem_base + lanes + TMEM_O + t * DIM;
+    uint32_t steps = 0, uses = 0, ring = 0, meetings = 0;  // ring: key and value tiles before this unit's
+    // (not a hardware barrier: a warp that gave up does not come again, and the others must not wait for ever)
+    auto all_meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(meet);
+      if (ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(meet, meetings & 1, SITE_PPRE_MEET));
+      ++meetings;
+    };
+    while (const Work* w = next_work()) {
+      const int j0 = w->j0, n = w->n_row[t], len = w->len;
       float m = neg_inf(), l = 0.f;
-      for (int j = j0; j < n[t]; ++j) {
-        if (ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(&s_full[t], (j - j0) & 1, SITE_PPRE_S));
-        if (!ok) break;
-        pre::tc_fence_after();
-        uint32_t x[TILE];
+      {
+        const int tok = w->tok0 + t * p.toks + row / p.group;
+        const int limit = row / p.group < p.toks && tok < w->q_len ? len - w->q_len + tok : -1;    // last slot this row sees
+        for (int j = j0; j < n; ++j) {
+          if (ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(&s_full[t], steps & 1, SITE_PPRE_S));
+          ++steps;
+          if (!ok) break;
+          pre::tc_fence_after();
+          uint32_t x[TILE];
 #pragma unroll
-        for (int c = 0; c < TILE; c += 32) tmem_ld32_issue(ts + c, x + c);
-        tmem_ld_wait();
-        const int last = limit - j * TILE;                 // last visible column
-        if (!__all_sync(0xffffffffu, last >= TILE - 1)) {
+          for (int c = 0; c < TILE; c += 32) tmem_ld32_issue(ts + c, x + c);
+          tmem_ld_wait();
+          const int last = limit - j * TILE;               // last visible column
+          if (!__all_sync(0xffffffffu, last >= TILE - 1)) {
 #pragma unroll
-          for (int c = 0; c < TILE; ++c) x[c] = c <= last ? x[c] : 0xff800000u;
-        }
-        float top[4];
+            for (int c = 0; c < TILE; ++c) x[c] = c <= last ? x[c] : 0xff800000u;
+          }
+          float top[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(x[i]);
+          for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(x[i]);
 #pragma unroll
-        for (int c = 4; c < TILE; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(x[c]));
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-        if (__any_sync(0xffffffffu, mx > m + GROWTH)) {
-          const float a = mx > m ? ex2(m - mx) : 1.f;      // (m still minus infinity: zero)
-          m = fmaxf(m, mx);
-          l *= a;
-          if (j > j0) {
+          for (int c = 4; c < TILE; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(x[c]));
+          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+          if (__any_sync(0xffffffffu, mx > m + GROWTH)) {
+            const float a = mx > m ? ex2(m - mx) : 1.f;    // (m still minus infinity: zero)
+            m = fmaxf(m, mx);
+            l *= a;
+            if (j > j0) {
 #pragma unroll
-            for (int c = 0; c < DIM; c += 32) {
-              uint32_t o[32];
-              tmem_ld32_issue(to + c, o);
-              tmem_ld_wait();
+              for (int c = 0; c < DIM; c += 16) {
+                uint32_t o[16];
+                csum::tmem_ld16(to + c, o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-              pre::tmem_st32(to + c, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                tmem_st16(to + c, o);
+              }
             }
           }
-        }
-        const float base = m == neg_inf() ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float base = m == neg_inf() ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < TILE; c += 64) {
-          uint32_t w[32];
+          for (int c = 0; c < TILE; c += 64) {
+            uint32_t wt[32];
 #pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            const float p0 = ex2(fmaf(__uint_as_float(x[c + i]), p.scale_log2, -base));
-            const float p1 = ex2(fmaf(__uint_as_float(x[c + i + 1]), p.scale_log2, -base));
-            sum[i & 2] += p0;
-            sum[(i & 2) + 1] += p1;
-            w[i / 2] = pack2<T>(p0, p1);
+            for (int i = 0; i < 64; i += 2) {
+              const float p0 = ex2(fmaf(__uint_as_float(x[c + i]), p.scale_log2, -base));
+              const float p1 = ex2(fmaf(__uint_as_float(x[c + i + 1]), p.scale_log2, -base));
+              sum[i & 2] += p0;
+              sum[(i & 2) + 1] += p1;
+              wt[i / 2] = pack2<T>(p0, p1);
+            }
+            pre::tmem_st32(ts + c / 2, wt);
           }
-          pre::tmem_st32(ts + c / 2, w);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if ((j + 1) * TILE > q.len) {
-          // the sequence ends in this tile: values behind it become zero before a product reads them
-          const int k = 2 * (j - j0) + 1, s = k % L::STAGES;
-          ok = __all_sync(0xffffffffu, wide::wait_suspend(&full[s], (k / L::STAGES) & 1, SITE_PPRE_VZERO));
-          if (!ok) break;
-          if (j * TILE + row >= q.len) {
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          if ((j + 1) * TILE > len) {
+            // the sequence ends in this tile: values behind it become zero before a product reads them
+            const uint32_t k = ring + 2 * (j - j0) + 1, s = k % L::STAGES;
+            ok = __all_sync(0xffffffffu, wide::wait_suspend(&full[s], (k / L::STAGES) & 1, SITE_PPRE_VZERO));
+            if (!ok) break;
+            if (j * TILE + row >= len) {
 #pragma unroll
-            for (int ch = 0; ch < DIM / 8; ++ch)
-              sts_v4(smem_u32(sm) + s * L::SLOT + (ch >> 3) * TILE * 128 + row * 128 + ((ch & 7) << 4), make_uint4(0, 0, 0, 0));
+              for (int ch = 0; ch < DIM / 8; ++ch)
+                sts_v4(smem_u32(sm) + s * L::SLOT + (ch >> 3) * TILE * 128 + row * 128 + ((ch & 7) << 4), make_uint4(0, 0, 0, 0));
+            }
+            fence_proxy_async_smem();
           }
-          fence_proxy_async_smem();
+          pre::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t]);
         }
+      }
+      ring += 2 * (max(w->n_row[0], w->n_row[1]) - j0);
+      // ------------------------------------------------------------ output
+      const bool any = n > j0;
+      if (any && ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(&o_full[t], uses & 1, SITE_PPRE_O));
+      if (any) ++uses;
+      pre::tc_fence_after();
+      const int tok = w->tok0 + t * p.toks + row / p.group;
+      const bool live = row / p.group < p.toks && tok < w->q_len;
+      const long long tr = w->q0 + tok;
+      const int hd = w->head * p.group + row % p.group;
+      T* dst_row = static_cast<T*>(p.out) + tr * p.o_tok + (long long)hd * p.o_head;
+      auto write_row = [&](int c, const float (&o)[16], float f) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 8)
+          reinterpret_cast<uint4*>(dst_row + c)[i / 8] = make_uint4(pack2<T>(o[i] * f, o[i + 1] * f), pack2<T>(o[i + 2] * f, o[i + 3] * f),
+                                                                    pack2<T>(o[i + 4] * f, o[i + 5] * f), pack2<T>(o[i + 6] * f, o[i + 7] * f));
+      };
+      auto write_lse = [&]() {
+        if (p.lse) p.lse[tr * p.n_heads + hd] = l > 0.f ? (m + log2f(l)) * LN2 : l == l ? neg_inf() : l;
+      };
+      const int pr = t * ROWS + row;                       // row of a part
+      float* part = p.parts + (long long)w->part * L::PART;
+      const bool whole = w->whole;
+      const float f = l > 0.f ? 1.f / l : 1.f;
+#pragma unroll
+      for (int c = 0; c < DIM; c += 16) {
+        uint32_t x[16];
+        float o[16];
+        if (any && ok) csum::tmem_ld16(to + c, x);
+        // where nothing was summed (or a NaN was) what the accumulator holds does not count; a NaN stays one
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = l > 0.f ? __uint_as_float(x[i]) : l;
+        if (whole) {
+          if (live && ok) write_row(c, o, f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            reinterpret_cast<float4*>(part + 4 * ROWS)[(c + i) / 4 * (2 * ROWS) + pr] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+      if (any) {
         pre::tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&o_empty[t]);
       }
-      // ------------------------------------------------------------ output
-      const int hd = head * p.group + row % p.group;
-      const bool any = n[t] > j0;
-      if (any && ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(&o_full[t], 0, SITE_PPRE_O));
-      if (ok) {
-        pre::tc_fence_after();
-        const long long tr = q.q0 + tok;
-        const float inv = l > 0.f ? 1.f / l : 0.f;         // a row that sees nothing is zero
-        const long long idx = ((long long)split * p.s.T + tr) * p.n_heads + hd;
-        if (live) {
-          if (p.splits > 1) {
-            *reinterpret_cast<float2*>(p.parts_ml + 2 * idx) = make_float2(m, l);
-          } else if (p.lse) {
-            p.lse[tr * p.n_heads + hd] = l > 0.f ? (m + log2f(l)) * LN2 : neg_inf();
-          }
+      if (whole) {
+        if (live && ok) write_lse();
+      } else {
+        reinterpret_cast<float2*>(part)[pr] = make_float2(m, l);
+        const int parts = w->parts;
+        const long long c0 = w->first_run;
+        __threadfence();
+        all_meet();
+        if (tid == 0) {
+          int* a = p.arrived + c0;                         // (at most one unit is cut for the first time in a run)
+          const bool is_last = atomicAdd(a, 1) == parts - 1;
+          if (is_last) *a = 0;
+          __threadfence();
+          *last_flag = is_last;
         }
+        all_meet();
+        if (ok && *last_flag && live) {
+          // the first part is the second of its run's two (the unit begins in that run), the others their run's first
+          auto part_of = [&](int k) { return p.parts + (2 * (c0 + k) + (k == 0 ? 1 : 0)) * L::PART; };
+          auto ml_of = [&](int k) { return __ldcg(reinterpret_cast<const float2*>(part_of(k)) + pr); };
+          m = neg_inf();
+          for (int k = 0; k < parts; ++k) m = fmaxf(m, ml_of(k).x);
+          l = 0.f;
+          float acc[DIM];
 #pragma unroll
-        for (int c = 0; c < DIM; c += 32) {
-          uint32_t o[32];
-          if (any) {
-            tmem_ld32_issue(to + c, o);
-            tmem_ld_wait();
+          for (int c = 0; c < DIM; ++c) acc[c] = 0.f;
+          for (int k = 0; k < parts; ++k) {
+            const float2 v = ml_of(k);
+            const float a = v.x == neg_inf() ? (v.y == v.y ? 0.f : 1.f) : ex2(v.x - m);
+            l += a * v.y;
+            const float4* src = reinterpret_cast<const float4*>(part_of(k) + 4 * ROWS) + pr;
+#pragma unroll
+            for (int c = 0; c < DIM; c += 4) {
+              const float4 o = __ldcg(src + c / 4 * (2 * ROWS));
+              acc[c] += a * o.x;
+              acc[c + 1] += a * o.y;
+              acc[c + 2] += a * o.z;
+              acc[c + 3] += a * o.w;
+            }
           }
-          if (!live) continue;
-          if (!(l > 0.f)) {
-            // nothing was summed (or a NaN was): what the accumulator holds does not count, a NaN stays one
+          const float g = l > 0.f ? 1.f / l : 1.f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = l == l ? 0u : 0x7fffffffu;
+          for (int c = 0; c < DIM; c += 16) {
+            float o[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = acc[c + i];
+            write_row(c, o, g);
           }
-          if (p.splits > 1) {
-            float4* dst = reinterpret_cast<float4*>(p.parts + idx * DIM + c);
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              dst[i / 4] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tr * p.o_tok + (long long)hd * p.o_head + c);
-            const float f = l == l ? inv : 1.f;
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              dst[i / 8] = make_uint4(pack2<T>(__uint_as_float(o[i]) * f, __uint_as_float(o[i + 1]) * f), pack2<T>(__uint_as_float(o[i + 2]) * f, __uint_as_float(o[i + 3]) * f),
-                                      pack2<T>(__uint_as_float(o[i + 4]) * f, __uint_as_float(o[i + 5]) * f), pack2<T>(__uint_as_float(o[i + 6]) * f, __uint_as_float(o[i + 7]) * f));
-          }
+          write_lse();
         }
       }
+      work_done();
     }
   }
   // Common exit, then the allocating warp frees tensor memory.  After a wait that gave up copies and MMAs may still be
@@ -420,38 +674,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     pre::tc_fence_after();
     pre::tmem_dealloc(tmem_base, TMEM_COLS);
   }
-}
-
-// Joins the splits of the kernel above: a warp per (token, head), in the order of the splits.
-template <typename T, int DIM>
-__global__ void __launch_bounds__(256) paged_join_kernel(const Params p) {
-  grid_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (long long)p.s.T * p.n_heads;
-  grid_dependency_wait();
-  if (row >= rows) return;
-  const int t = (int)(row / p.n_heads), hd = (int)(row % p.n_heads);
-  int below = 0;
-  for (int i = lane; i <= p.s.n; i += 32) below += ld_plain(p.s.cu + i) <= t;
-  const int b = __reduce_add_sync(0xffffffffu, below) - 1;
-  if (b < 0 || b >= p.s.n) return;
-  const Seq q = load_seq(p.s, b);
-  if (seq_blocks(p, q) == 0 || t >= q.q0 + q.q_len) return;
-  constexpr int E = DIM / 32;
-  float m = neg_inf(), l = 0.f, acc[E] = {};
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.parts_ml[2 * (s * rows + row)]);
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.parts_ml + 2 * (s * rows + row));
-    const float a = ml.x == neg_inf() ? (ml.y == ml.y ? 0.f : 1.f) : ex2(ml.x - m);
-    l += a * ml.y;
-#pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] += a * p.parts[(s * rows + row) * DIM + lane * E + i];
-  }
-  const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : 1.f;
-  T* dst = static_cast<T*>(p.out) + (long long)t * p.o_tok + (long long)hd * p.o_head + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
-  if (p.lse && lane == 0) p.lse[row] = l > 0.f ? (m + log2f(l)) * LN2 : l == l ? neg_inf() : l;
 }
 
 }  // namespace ppre
