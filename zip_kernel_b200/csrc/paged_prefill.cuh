@@ -48,7 +48,7 @@ struct Layout {
   static constexpr int q = STAGES * SLOT;
   static constexpr int works = q + 2 * SLOT;                 // Work [WORKS]
   static constexpr int bars = works + WORKS * 64;
-  static constexpr int total = bars + (2 * STAGES + 13 + 2 * WORKS) * 8 + 16;
+  static constexpr int total = bars + (2 * STAGES + 15 + 2 * WORKS) * 8 + 16;
   static constexpr int PART = 2 * ROWS * (DIM + 2);          // of a unit in the workspace: float2 m, l [row], float4 [dim / 4][row]
   static_assert(1024 + total <= 232448, "shared memory of one SM");
 };
@@ -69,7 +69,7 @@ struct Params {
 // A unit is a pair of row tiles of one (sequence, key/value head).  All units lie end to end, measured in slots: those that
 // a unit's last row sees and PAD more for what a unit costs besides its tiles; the row is cut into one equal run per
 // CTA.  A unit that falls into several runs is joined by the CTA that finishes its last part, in the order of the parts.
-constexpr int PAD = 192;
+constexpr int PAD = 320;
 constexpr int MIN_RUN = 4 * TILE;                            // shorter runs cost more in joining than they save
 
 struct Unit {
@@ -227,6 +227,57 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// Largest of three; NaN when one is (unlike fmaxf)
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2_t add_f32x2(f32x2_t a, f32x2_t b) {
+  f32x2_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2^x for two x in [-126, 126] on the multiply-add pipe: x = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 leaves n
+// in the low bits), 2^f by a polynomial of degree 4 (largest relative error 2.6e-6, fitted to that by reweighted least
+// squares), n added to the exponent.
+__device__ __forceinline__ float2 ex2_poly(f32x2_t x) {
+  const f32x2_t big = pack_f32x2(12582912.f, 12582912.f), neg_big = pack_f32x2(-12582912.f, -12582912.f), minus = pack_f32x2(-1.f, -1.f);
+  const f32x2_t t = add_f32x2(x, big);
+  const f32x2_t f = fma_f32x2(add_f32x2(t, neg_big), minus, x);
+  f32x2_t y = fma_f32x2(f, pack_f32x2(0.009570101276040077f, 0.009570101276040077f), pack_f32x2(0.05591785907745361f, 0.05591785907745361f));
+  y = fma_f32x2(f, y, pack_f32x2(0.240247443318367f, 0.240247443318367f));
+  y = fma_f32x2(f, y, pack_f32x2(0.6931217908859253f, 0.6931217908859253f));
+  y = fma_f32x2(f, y, pack_f32x2(0.9999992847442627f, 0.9999992847442627f));
+  const float2 n = unpack_f32x2(t), r = unpack_f32x2(y);
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(r.y) + (__float_as_int(n.y) << 23)));
+}
+
+// The weights 2^(x * scale - base) of half a row's scores, as 16-bit pairs to tensor memory; returns their sum.  The unit
+// for 2^x makes 4 a clock and scheduler, as many clocks for both row tiles as their products take, and one warp does not
+// hide the rest behind it: FAST, one pair of three goes through the multiply-add pipe, whose polynomial takes no NaN or
+// infinity.  Measured, 128 columns by one warp a scheduler: 1269 clocks with none, 1093 with one of four, 1045 with
+// one of three, 1055 with one of two.
+constexpr int POLY_OF = 3;
+template <typename T, bool FAST>
+__device__ __forceinline__ float half_weights(const uint32_t* x, float scale, float base, uint32_t tp) {
+  const f32x2_t scale2 = pack_f32x2(scale, scale), base2 = pack_f32x2(-base, -base);
+  f32x2_t sum[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
+  uint32_t w[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const f32x2_t v = fma_f32x2(pack_f32x2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, base2);
+    float2 e = unpack_f32x2(v);
+    if (FAST && i % POLY_OF == POLY_OF - 1) e = ex2_poly(pack_f32x2(fmaxf(e.x, -126.f), fmaxf(e.y, -126.f)));
+    else e = make_float2(ex2(e.x), ex2(e.y));
+    sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e.x, e.y));
+    w[i] = pack2<T>(e.x, e.y);
+  }
+  pre::tmem_st32(tp, w);
+  const float2 s = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+  return s.x + s.y;
+}
+
 // Bounded wait that never sleeps, for the thread that issues the MMAs: it wakes from a sleeping wait about 450 clocks after
 // the arrival, and every hand-over between products and softmax would pay that.
 __device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity, int site) {
@@ -257,8 +308,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   uint64_t* q_full = empty + L::STAGES;                          // [2] per row tile, as the next five
   uint64_t* q_empty = q_full + 2;
   uint64_t* s_full = q_empty + 2;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
+  uint64_t* p_full = s_full + 2;                                 // [2][2 halves of the slots]
+  uint64_t* o_full = p_full + 4;
   uint64_t* o_empty = o_full + 2;
   uint64_t* w_full = o_empty + 2;                                // [WORKS]
   uint64_t* w_empty = w_full + WORKS;
@@ -273,7 +324,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_empty[i], 4);
     }
@@ -446,18 +498,22 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           bool k_here = false;
           for (int t = 0; ok && t < 2; ++t) {
             if (j >= n_row[t]) continue;
-            ok = wait_spin(&p_full[t], steps[t] & 1, SITE_PPRE_P);
-            ++steps[t];
-            if (ok && j == j0) {                           // the output of the unit before has been read
+            if (j == j0) {                                 // the output of the unit before has been read
               if (uses[t] > 0) ok = wide::wait_suspend(&o_empty[t], (uses[t] - 1) & 1, SITE_PPRE_OEMPTY);
               ++uses[t];
             }
-            if (!ok) break;
-            pre::tc_fence_after();
             const uint64_t bd = smem_desc_mn_sw128(smem_u32(sm + vs * L::SLOT), TILE * 128);
 #pragma unroll
-            for (int k = 0; k < TILE / 16; ++k)
-              umma_f16_ta(tmem_base + TMEM_O + t * DIM, tmem_base + t * TILE + k * 8, bd + k * (2048 >> 4), j > j0 || k > 0, id_o);
+            for (int h = 0; h < 2; ++h) {
+              if (ok) ok = wait_spin(&p_full[2 * t + h], steps[t] & 1, SITE_PPRE_P);
+              if (!ok) break;
+              pre::tc_fence_after();
+#pragma unroll
+              for (int k = h * 4; k < h * 4 + 4; ++k)
+                umma_f16_ta(tmem_base + TMEM_O + t * DIM, tmem_base + t * TILE + k * 8, bd + k * (2048 >> 4), j > j0 || k > 0, id_o);
+            }
+            if (!ok) break;
+            ++steps[t];
             if (j == n_row[t] - 1) pre::umma_commit(&o_full[t]);
             if (j + 1 < n_row[t]) {
               if (!k_here) ok = wait_spin(&full[ks], kph, SITE_PPRE_K);
@@ -495,6 +551,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       {
         const int tok = w->tok0 + t * p.toks + row / p.group;
         const int limit = row / p.group < p.toks && tok < w->q_len ? len - w->q_len + tok : -1;    // last slot this row sees
+        const int limit_all = __reduce_min_sync(0xffffffffu, limit);
         for (int j = j0; j < n; ++j) {
           if (ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(&s_full[t], steps & 1, SITE_PPRE_S));
           ++steps;
@@ -504,8 +561,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
           for (int c = 0; c < TILE; c += 32) tmem_ld32_issue(ts + c, x + c);
           tmem_ld_wait();
-          const int last = limit - j * TILE;               // last visible column
-          if (!__all_sync(0xffffffffu, last >= TILE - 1)) {
+          const bool clear = (j + 1) * TILE - 1 <= limit_all;
+          if (!clear) {
+            const int last = limit - j * TILE;             // last visible column
 #pragma unroll
             for (int c = 0; c < TILE; ++c) x[c] = c <= last ? x[c] : 0xff800000u;
           }
@@ -513,39 +571,34 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
           for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(x[i]);
 #pragma unroll
-          for (int c = 4; c < TILE; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(x[c]));
-          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-          if (__any_sync(0xffffffffu, mx > m + GROWTH)) {
-            const float a = mx > m ? ex2(m - mx) : 1.f;    // (m still minus infinity: zero)
-            m = fmaxf(m, mx);
-            l *= a;
-            if (j > j0) {
+          for (int c = 4; c + 8 <= TILE; c += 8)
 #pragma unroll
-              for (int c = 0; c < DIM; c += 16) {
-                uint32_t o[16];
-                csum::tmem_ld16(to + c, o);
+            for (int i = 0; i < 4; ++i) top[i] = max3_nan(top[i], __uint_as_float(x[c + i]), __uint_as_float(x[c + 4 + i]));
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-                tmem_st16(to + c, o);
+          for (int i = 0; i < 4; ++i) top[i] = max3_nan(top[i], __uint_as_float(x[TILE - 4 + i]), neg_inf());
+          const float all_top = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], neg_inf());
+          const float mx = all_top * p.scale_log2;         // (a NaN leaves the maximum alone and the weights are NaN)
+          // one vote a tile: some row's maximum has grown, or some score is not finite
+          bool fast = clear;
+          if (__any_sync(0xffffffffu, !(mx <= m + GROWTH) || !(mx > -3e38f))) {
+            fast = clear && __all_sync(0xffffffffu, fabsf(mx) < 3e38f);
+            if (__any_sync(0xffffffffu, mx > m + GROWTH)) {
+              const float a = mx > m ? ex2(m - mx) : 1.f;  // (m still minus infinity: zero)
+              m = fmaxf(m, mx);
+              l *= a;
+              if (j > j0) {
+#pragma unroll
+                for (int c = 0; c < DIM; c += 16) {
+                  uint32_t o[16];
+                  csum::tmem_ld16(to + c, o);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                  tmem_st16(to + c, o);
+                }
               }
             }
           }
           const float base = m == neg_inf() ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < TILE; c += 64) {
-            uint32_t wt[32];
-#pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(x[c + i]), p.scale_log2, -base));
-              const float p1 = ex2(fmaf(__uint_as_float(x[c + i + 1]), p.scale_log2, -base));
-              sum[i & 2] += p0;
-              sum[(i & 2) + 1] += p1;
-              wt[i / 2] = pack2<T>(p0, p1);
-            }
-            pre::tmem_st32(ts + c / 2, wt);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           if ((j + 1) * TILE > len) {
             // the sequence ends in this tile: values behind it become zero before a product reads them
             const uint32_t k = ring + 2 * (j - j0) + 1, s = k % L::STAGES;
@@ -558,9 +611,16 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             }
             fence_proxy_async_smem();
           }
+          // The product with the first 64 slots' values starts while the other weights are made; it reads only rows of
+          // values that this warp's row tile has zeroed where need be (all four warps arrive for either half).
+          l += fast ? half_weights<T, true>(x, p.scale_log2, base, ts) : half_weights<T, false>(x, p.scale_log2, base, ts);
           pre::tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t]);
+          if (lane == 0) mbar_arrive(&p_full[2 * t]);
+          l += fast ? half_weights<T, true>(x + 64, p.scale_log2, base, ts + 32) : half_weights<T, false>(x + 64, p.scale_log2, base, ts + 32);
+          pre::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + 1]);
         }
       }
       ring += 2 * (max(w->n_row[0], w->n_row[1]) - j0);
