@@ -232,10 +232,10 @@ def workspace(device: torch.device, T: int, K: int, N: int, nnz: int) -> torch.T
     return buf
 
 
-def attention_workspace(kv, T: int, n_heads: int, max_q_len: int) -> torch.Tensor:
+def attention_workspace(kv, T: int, n_heads: int, max_q_len: int, stream: int) -> torch.Tensor:
     """Scratch of the attention on a paged cache: apart from the linears' because its counters start, and end, as zeros."""
     need = int(load().w4a4_paged_attention_workspace_bytes(kv._ptr, T, n_heads, max_q_len))
-    key = (kv.device.index, stream_ptr(kv.device), "attention")
+    key = (kv.device.index, stream, "attention")
     holder = getattr(_tls, "holder", None)
     if holder is not None:
         return holder.get(key, need, kv.device)

@@ -2,14 +2,15 @@
 // last `recent` ones and those with the largest sums in between, `budget` in all (equal sums: the lowest slots), move in
 // their order to the slots 0, 1, ... of the destination.  A sequence of at most `budget` slots keeps them all.
 //
-// Two launches.  select: a block per (sequence, head) finds the smallest sum that stays by a radix selection, eight bits
-// of an order-preserving integer form of the float at a time, then walks the slots once in order and writes the list of
+// Two launches.  select: a block per (sequence, head) finds the smallest sum that stays by a radix selection, 11, 11 and 10
+// bits of an order-preserving integer form of the float at a time, then walks the slots once in order and writes the list of
 // those kept and their sums.  move: copies the rows of the list.  In place a row's new slot is never above its old one,
 // so rows may be written in ascending order once all rows up to them have been read; the columns of a row are
 // independent of one another, and a block takes a few columns of all rows of one (sequence, head).  Into another cache
 // the rows are independent too and are split over blocks.
 //
-// What bounds it: the rows kept are read and written once; the selection reads the sums six times, from L2 after the first.
+// What bounds it: the rows kept are read and written once; the selection holds up to 8192
+// sums in registers and reads longer ones again from L2.
 #pragma once
 
 #include "paged_kv.cuh"
@@ -19,7 +20,8 @@ namespace evict {
 
 using namespace kv;
 
-constexpr int SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, BINS = 256;
+constexpr int SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, BINS = 2048;
+constexpr int KEYS = 8;                                      // keys a thread holds; longer sequences are read again every pass
 constexpr int MOVE_THREADS = 256, MOVE_CHUNKS = 8, MOVE_UNROLL = 8, MOVE_ROWS = MOVE_THREADS / MOVE_CHUNKS * MOVE_UNROLL;
 static_assert(MOVE_ROWS == MOVE_THREADS, "a thread locates one row of a batch");
 
@@ -41,10 +43,9 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 
 __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const SelectParams p) {
-  __shared__ int hist[SELECT_WARPS][BINS];
-  __shared__ int warp_sums[2][SELECT_WARPS];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
+  __shared__ int hist[BINS];
+  __shared__ int warp_sums[2][2][SELECT_WARPS];
+  __shared__ int s_bin, s_left, s_count;
   grid_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.x / p.n_kv, g = blockIdx.x % p.n_kv;
@@ -65,74 +66,87 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Sele
   } else {
     const int lo = p.sink, hi = n - p.recent;              // candidates; the rest stays anyway (sink + recent <= budget < n)
     int left = p.budget - p.sink - p.recent;               // how many of them stay
-    uint32_t prefix = 0;                                   // leading bits of the smallest key that stays
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < SELECT_WARPS * BINS; i += SELECT_THREADS) hist[i / BINS][i % BINS] = 0;
-      __syncthreads();
-      for (int j = lo + tid; j < hi; j += SELECT_THREADS) {
-        const uint32_t k = order_key(ld_plain(sums + j));
-        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[warp][(k >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (tid < BINS) {
-        int s = 0;
-        for (int k = 0; k < SELECT_WARPS; ++k) s += hist[k][tid];
-        hist[0][tid] = s;
-      }
-      __syncthreads();
-      if (warp == 0) {
-        // bins from the top: the one in which the count reaches `left`
-        int mine[8], s = 0;
+    const bool any = left > 0, held = n <= KEYS * SELECT_THREADS;
+    float v[KEYS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { mine[i] = hist[0][255 - (lane * 8 + i)]; s += mine[i]; }
-        int above = s;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-          const int a = __shfl_up_sync(0xffffffffu, above, o);
-          if (lane >= o) above += a;
-        }
-        above -= s;                                        // of the lanes before
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (above < left && left <= above + mine[i]) {
-            s_prefix = prefix | ((uint32_t)(255 - (lane * 8 + i)) << shift);
-            s_left = left - above;
-          }
-          above += mine[i];
-        }
-      }
-      __syncthreads();
-      if (left > 0) { prefix = s_prefix; left = s_left; }
+    for (int i = 0; i < KEYS; ++i) {
+      const int j = i * SELECT_THREADS + tid;
+      v[i] = held && j < n ? ld_plain(sums + j) : 0.f;
     }
-    // Now `prefix` is the smallest key that stays, `left` how many slots with just that key do: the first ones.
-    const bool any = p.budget > p.sink + p.recent;
-    int done = 0, ties = 0;                                // slots kept, and slots with that key, before this round
-    for (int base = 0; base < n; base += SELECT_THREADS) {
-      const int j = base + tid;
+    uint32_t prefix = 0;                                   // leading bits of the smallest key that stays
+#pragma unroll 1
+    for (int pass = 0; any && pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < BINS; i += SELECT_THREADS) hist[i] = 0;
+      __syncthreads();
+      auto count = [&](int j, float x) {
+        if (j < lo || j >= hi) return;
+        const uint32_t k = order_key(x);
+        if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
+      };
+      if (held) {
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) count(i * SELECT_THREADS + tid, v[i]);
+      } else {
+        for (int j = lo + tid; j < hi; j += SELECT_THREADS) count(j, ld_plain(sums + j));
+      }
+      __syncthreads();
+      // bins from the top, two a thread: the one in which the count reaches `left`
+      const int h0 = hist[BINS - 1 - 2 * tid], h1 = hist[BINS - 2 - 2 * tid];
+      int above = h0 + h1;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int a = __shfl_up_sync(0xffffffffu, above, o);
+        if (lane >= o) above += a;
+      }
+      if (lane == 31) warp_sums[0][0][warp] = above;
+      __syncthreads();
+      above += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[0][0][lane] : 0) - h0 - h1;
+      if (above < left && left <= above + h0 + h1) {
+        const bool second = left > above + h0;
+        s_bin = BINS - 1 - 2 * tid - (second ? 1 : 0);
+        s_left = left - above - (second ? h0 : 0);
+        s_count = second ? h1 : h0;
+      }
+      __syncthreads();
+      prefix |= (uint32_t)s_bin << shift;
+      left = s_left;
+      if (left == s_count) break;                          // the whole bin stays: its lowest key is the border
+    }
+    // Now `prefix` is the smallest key that stays, or below it and above all that go, and `left` how many slots with
+    // just that leading part stay: the first ones.
+    int done = 0, ties = 0;                                // slots kept, and slots with the border's key, before this round
+    auto place = [&](int j, float x, int round) {
       bool sure = false, tie = false;
-      float v = 0.f;
       if (j < n) {
-        v = ld_plain(sums + j);
-        const uint32_t k = order_key(v);
+        const uint32_t k = order_key(x);
         const bool free = j >= lo && j < hi;
         sure = !free || (any && k > prefix);
         tie = free && any && k == prefix;
       }
       const unsigned ms = __ballot_sync(0xffffffffu, sure), mt = __ballot_sync(0xffffffffu, tie), before = (1u << lane) - 1;
-      if (lane == 0) { warp_sums[0][warp] = __popc(ms); warp_sums[1][warp] = __popc(mt); }
+      int(*sums_of)[SELECT_WARPS] = warp_sums[round & 1];  // (two in turn: one barrier a round)
+      if (lane == 0) { sums_of[0][warp] = __popc(ms); sums_of[1][warp] = __popc(mt); }
       __syncthreads();
-      const int ws = warp_sums[0][lane], wt = warp_sums[1][lane];
+      const int ws = sums_of[0][lane], wt = sums_of[1][lane];
       const int s_before = __reduce_add_sync(0xffffffffu, lane < warp ? ws : 0) + __popc(ms & before);
       const int t_before = ties + __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0) + __popc(mt & before);
       const int s_all = __reduce_add_sync(0xffffffffu, ws), t_all = __reduce_add_sync(0xffffffffu, wt);
       if (sure || (tie && t_before < left)) {
         const int to = done + s_before + min(t_before, left) - min(ties, left);
         kept[to] = j;
-        out[to] = v;
+        out[to] = x;
       }
       done += s_all + min(ties + t_all, left) - min(ties, left);
       ties += t_all;
-      __syncthreads();
+    };
+    __syncthreads();
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i)
+        if (i * SELECT_THREADS < n) place(i * SELECT_THREADS + tid, v[i], i);
+    } else {
+      for (int base = 0, r = 0; base < n; base += SELECT_THREADS, ++r) place(base + tid, base + tid < n ? ld_plain(sums + base + tid) : 0.f, r);
     }
   }
   for (int j = n_new + tid; j < p.budget; j += SELECT_THREADS) kept[j] = -1;

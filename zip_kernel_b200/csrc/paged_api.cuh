@@ -189,8 +189,14 @@ int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long l
   // one token a block while blocks are few, for the latency of a decode step; then four, which pay for the chain to
   // the page number once
   p.toks = T > 8 * dev->sm_count ? 4 : T > 4 * dev->sm_count ? 2 : 1;
-  auto kern = cache->head_dim == 128 ? by_type(cache->dtype, kv::qkv_rope_kernel<__half, 128>, kv::qkv_rope_kernel<__nv_bfloat16, 128>)
-                                     : by_type(cache->dtype, kv::qkv_rope_kernel<__half, 64>, kv::qkv_rope_kernel<__nv_bfloat16, 64>);
+  auto pick = [&](auto k64h, auto k64b, auto k128h, auto k128b) { return cache->head_dim == 128 ? by_type(cache->dtype, k128h, k128b) : by_type(cache->dtype, k64h, k64b); };
+  auto kern = interleaved ? pick(kv::qkv_rope_kernel<__half, 64, kv::ROPE_PAIRS>, kv::qkv_rope_kernel<__nv_bfloat16, 64, kv::ROPE_PAIRS>,
+                                 kv::qkv_rope_kernel<__half, 128, kv::ROPE_PAIRS>, kv::qkv_rope_kernel<__nv_bfloat16, 128, kv::ROPE_PAIRS>)
+              : rot_dim == cache->head_dim
+                  ? pick(kv::qkv_rope_kernel<__half, 64, kv::ROPE_HALVES>, kv::qkv_rope_kernel<__nv_bfloat16, 64, kv::ROPE_HALVES>,
+                         kv::qkv_rope_kernel<__half, 128, kv::ROPE_HALVES>, kv::qkv_rope_kernel<__nv_bfloat16, 128, kv::ROPE_HALVES>)
+                  : pick(kv::qkv_rope_kernel<__half, 64, kv::ROPE_APART>, kv::qkv_rope_kernel<__nv_bfloat16, 64, kv::ROPE_APART>,
+                         kv::qkv_rope_kernel<__half, 128, kv::ROPE_APART>, kv::qkv_rope_kernel<__nv_bfloat16, 128, kv::ROPE_APART>);
   cudaError_t e = launch_ex(kern, dim3((unsigned)((T + p.toks - 1) / p.toks)), dim3(kv::ROPE_THREADS), 0, static_cast<cudaStream_t>(stream), 1, p);
   if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "rope kernel launch: %s", cudaGetErrorString(e));
   return W4A4_OK;
@@ -340,10 +346,18 @@ int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long 
   if (!rc) rc = make_query_map(&tq, q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim, cache->dtype, group, p.toks);
   if (rc) return rc;
   const bool d128 = cache->head_dim == 128;
-  auto kern = d128 ? by_type(cache->dtype, csum::cache_sums_kernel<__half, 128>, csum::cache_sums_kernel<__nv_bfloat16, 128>)
-                   : by_type(cache->dtype, csum::cache_sums_kernel<__half, 64>, csum::cache_sums_kernel<__nv_bfloat16, 64>);
-  cudaError_t e = launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(csum::THREADS), d128 ? csum::smem_bytes<128>() : csum::smem_bytes<64>(),
-                            static_cast<cudaStream_t>(stream), 1, tk, tq, p);
+  auto launch = [&](auto k64h, auto k64b, auto k128h, auto k128b, size_t smem) {
+    auto kern = d128 ? by_type(cache->dtype, k128h, k128b) : by_type(cache->dtype, k64h, k64b);
+    return launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(csum::THREADS), smem, static_cast<cudaStream_t>(stream), 1, tk, tq, p);
+  };
+  constexpr int N = csum::NARROW, M = csum::MAX_COLS;
+  const cudaError_t e =
+      p.cols <= N ? launch(csum::cache_sums_kernel<__half, 64, N>, csum::cache_sums_kernel<__nv_bfloat16, 64, N>,
+                           csum::cache_sums_kernel<__half, 128, N>, csum::cache_sums_kernel<__nv_bfloat16, 128, N>,
+                           d128 ? csum::smem_bytes<128, N>() : csum::smem_bytes<64, N>())
+                  : launch(csum::cache_sums_kernel<__half, 64, M>, csum::cache_sums_kernel<__nv_bfloat16, 64, M>,
+                           csum::cache_sums_kernel<__half, 128, M>, csum::cache_sums_kernel<__nv_bfloat16, 128, M>,
+                           d128 ? csum::smem_bytes<128, M>() : csum::smem_bytes<64, M>());
   if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "weight sums kernel launch: %s", cudaGetErrorString(e));
   return W4A4_OK;
 }

@@ -27,8 +27,10 @@ namespace w4a4 {
 namespace ppre {
 
 using namespace kv;
+using csum::add_f32x2;
 using csum::idesc_f16;
 using csum::umma_f16;
+using csum::wait_spin;
 
 constexpr int TILE = 128, ROWS = 128;                        // slots of a tile, rows of a row tile
 constexpr int WARP_COPY = 8, WARP_MMA = 9, WARP_PLAN = 10, THREADS = 12 * 32;
@@ -233,11 +235,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ f32x2_t add_f32x2(f32x2_t a, f32x2_t b) {
-  f32x2_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // 2^x for two x in [-126, 126] on the multiply-add pipe: x = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 leaves n
 // in the low bits), 2^f by a polynomial of degree 4 (largest relative error 2.6e-6, fitted to that by reweighted least
 // squares), n added to the exponent.
@@ -276,24 +273,6 @@ __device__ __forceinline__ float half_weights(const uint32_t* x, float scale, fl
   pre::tmem_st32(tp, w);
   const float2 s = unpack_f32x2(add_f32x2(sum[0], sum[1]));
   return s.x + s.y;
-}
-
-// Bounded wait that never sleeps, for the thread that issues the MMAs: it wakes from a sleeping wait about 450 clocks after
-// the arrival, and every hand-over between products and softmax would pay that.
-__device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity, int site) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (done) return true;
-    if ((i & 0xffff) == 0) {                               // (65536 polls are some milliseconds)
-      if (t0 == 0) t0 = wide::timer_ns();
-      else if (i > wide::WAIT_POLLS && wide::timer_ns() - t0 > wide::WAIT_NS) break;
-    }
-  }
-  record_error(site, parity);
-  return false;
 }
 
 template <typename T, int DIM>

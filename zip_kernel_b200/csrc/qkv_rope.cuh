@@ -37,11 +37,17 @@ struct RopeParams {
   float eps;
 };
 
+// How a lane's eight elements lie in the row and where the partner of each is.  In the two usual layouts pairs do not leave
+// the lane: PAIRS takes eight neighbours, HALVES four of either half of the row.  APART (halves of a part of the row)
+// takes eight neighbours and gets their partners from another lane.  Measured, 16384 tokens of 80 heads with norms,
+// halves: 172 us with partners from other lanes (eight exchanges per 16 bytes) and IEEE square root and division.
+enum : int { ROPE_PAIRS, ROPE_HALVES, ROPE_APART };
+
 // A block takes `toks` tokens, and each of them ROPE_THREADS / LANES / toks groups of LANES lanes that go through its
 // rows in turn with the token's cosines and sines in registers.
-template <typename T, int DIM>
+template <typename T, int DIM, int MODE>
 __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopeParams p) {
-  constexpr int LANES = DIM / 8, GROUPS = ROPE_THREADS / LANES, UNROLL = 4;
+  constexpr int LANES = DIM / 8, GROUPS = ROPE_THREADS / LANES, UNROLL = 4, ANGLES = MODE == ROPE_APART ? 8 : 4;
   grid_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31;
   const int sub = tid % LANES;               // this thread's 8 elements of a head row
@@ -49,7 +55,31 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopePar
   const int t = blockIdx.x * p.toks + tid / LANES / per_tok, row_first = tid / LANES % per_tok;
   if (t >= p.s.T) return;                    // (a warp's lanes share a token: a token has four groups or more)
   const int n_rows = p.n_heads + 2 * p.c.n_kv;
-  const T* src = static_cast<const T*>(p.qkv) + (long long)t * p.ld_qkv + sub * 8;
+  const T* src = static_cast<const T*>(p.qkv) + (long long)t * p.ld_qkv;
+  auto get = [&](const T* row) -> uint4 {
+    if (MODE == ROPE_HALVES) {
+      const uint2 a = ld_plain(reinterpret_cast<const uint2*>(row + sub * 4)), b = ld_plain(reinterpret_cast<const uint2*>(row + DIM / 2 + sub * 4));
+      return make_uint4(a.x, a.y, b.x, b.y);
+    }
+    return ld_plain(reinterpret_cast<const uint4*>(row + sub * 8));
+  };
+  auto put = [&](T* row, const uint4& v) {
+    if (MODE == ROPE_HALVES) {
+      *reinterpret_cast<uint2*>(row + sub * 4) = make_uint2(v.x, v.y);
+      *reinterpret_cast<uint2*>(row + DIM / 2 + sub * 4) = make_uint2(v.z, v.w);
+    } else {
+      *reinterpret_cast<uint4*>(row + sub * 8) = v;
+    }
+  };
+  auto floats = [&](const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 e = unpack2<T>(w[i]);
+      f[2 * i] = e.x;
+      f[2 * i + 1] = e.y;
+    }
+  };
   grid_dependency_wait();
 
   uint4 x[UNROLL];
@@ -57,7 +87,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopePar
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int r = row0 + u * per_tok + row_first;
-      if (r < n_rows) x[u] = ld_plain(reinterpret_cast<const uint4*>(src + (long long)r * DIM));
+      if (r < n_rows) x[u] = get(src + (long long)r * DIM);
     }
   };
   load(0);
@@ -76,22 +106,19 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopePar
   }
   const int page = page_of(p.c, b, slot / p.c.page), in_page = slot % p.c.page;
 
-  // cosines and sines of this thread's elements: four pairs of neighbours, or eight elements of one half
+  // cosines and sines of this thread's pairs
   const int half = p.rot / 2;
-  const bool rotated = sub * 8 < p.rot;
-  const int partner = p.interleaved ? 0 : (sub * 8 < half ? half / 8 : -(half / 8));
-  const int sub0 = p.interleaved ? sub * 4 : (sub * 8 < half ? sub * 8 : sub * 8 - half);
-  float cs[8] = {}, sn[8] = {};
+  const bool rotated = MODE == ROPE_HALVES || sub * 8 < p.rot;
+  const int partner = sub * 8 < half ? half / 8 : -(half / 8);
+  const int angle0 = MODE != ROPE_APART ? sub * 4 : (sub * 8 < half ? sub * 8 : sub * 8 - half);
+  float cs[ANGLES] = {}, sn[ANGLES] = {};
   if (rotated) {
-    const float* cp = p.cos + (long long)pos * half + sub0;
-    const float* sp = p.sin + (long long)pos * half + sub0;
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      if (i == 0 || !p.interleaved) {
-        const float4 c4 = ld_plain(reinterpret_cast<const float4*>(cp + i)), s4 = ld_plain(reinterpret_cast<const float4*>(sp + i));
-        cs[i] = c4.x; cs[i + 1] = c4.y; cs[i + 2] = c4.z; cs[i + 3] = c4.w;
-        sn[i] = s4.x; sn[i + 1] = s4.y; sn[i + 2] = s4.z; sn[i + 3] = s4.w;
-      }
+    for (int i = 0; i < ANGLES; i += 4) {
+      const float4 c4 = ld_plain(reinterpret_cast<const float4*>(p.cos + (long long)pos * half + angle0 + i));
+      const float4 s4 = ld_plain(reinterpret_cast<const float4*>(p.sin + (long long)pos * half + angle0 + i));
+      cs[i] = c4.x; cs[i + 1] = c4.y; cs[i + 2] = c4.z; cs[i + 3] = c4.w;
+      sn[i] = s4.x; sn[i + 1] = s4.y; sn[i + 2] = s4.z; sn[i + 3] = s4.w;
     }
   }
 
@@ -103,16 +130,8 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopePar
       uint4 y = live ? x[u] : make_uint4(0, 0, 0, 0);
       if (__any_sync(0xffffffffu, live && !is_v)) {
         float f[8];
-        {
-          const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 v = unpack2<T>(w[i]);
-            f[2 * i] = v.x;
-            f[2 * i + 1] = v.y;
-          }
-        }
-        const void* nw = is_q ? p.q_norm : p.k_norm;
+        floats(y, f);
+        const T* nw = static_cast<const T*>(is_q ? p.q_norm : p.k_norm);
         if (p.q_norm != nullptr || p.k_norm != nullptr) {
           float ss = 0.f;
 #pragma unroll
@@ -120,29 +139,23 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopePar
 #pragma unroll
           for (int o = LANES / 2; o > 0; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
           if (nw != nullptr) {
-            const float r_rms = 1.f / sqrtf(ss * (1.f / DIM) + p.eps);
-            const uint4 w4 = ld_plain(reinterpret_cast<const uint4*>(static_cast<const T*>(nw) + sub * 8));
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            const float r_rms = rsqrtf(ss * (1.f / DIM) + p.eps);      // (two steps of fp32 off at most)
+            float w[8];
+            floats(get(nw), w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 v = unpack2<T>(w[i]);
-              f[2 * i] *= r_rms * v.x;
-              f[2 * i + 1] *= r_rms * v.y;
-            }
+            for (int i = 0; i < 8; ++i) f[i] *= r_rms * w[i];
           }
         }
         float g[8];
-        if (p.interleaved) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            g[2 * i] = f[2 * i] * cs[i] - f[2 * i + 1] * sn[i];
-            g[2 * i + 1] = f[2 * i + 1] * cs[i] + f[2 * i] * sn[i];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; ++i) {
+          if (MODE == ROPE_PAIRS) {
+            g[i] = i & 1 ? f[i] * cs[i / 2] + f[i - 1] * sn[i / 2] : f[i] * cs[i / 2] - f[i + 1] * sn[i / 2];
+          } else if (MODE == ROPE_HALVES) {
+            g[i] = i >= 4 ? f[i] * cs[i - 4] + f[i - 4] * sn[i - 4] : f[i] * cs[i] - f[i + 4] * sn[i];
+          } else {
             const float o = __shfl_sync(0xffffffffu, f[i], (lane & ~(LANES - 1)) | ((sub + partner) & (LANES - 1)));
-            g[i] = f[i] * cs[i] + (partner > 0 ? -o : o) * sn[i];
+            g[i] = f[i] * cs[i % ANGLES] + (partner > 0 ? -o : o) * sn[i % ANGLES];
           }
         }
         if (!is_v) {
@@ -152,15 +165,13 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopePar
         }
       }
       if (live) {
-        T* dst = nullptr;
         if (is_q) {
-          dst = static_cast<T*>(p.q_out) + (long long)t * p.q_tok + (long long)r * p.q_head;
+          put(static_cast<T*>(p.q_out) + (long long)t * p.q_tok + (long long)r * p.q_head, y);
         } else if (page >= 0) {
           const int h = is_v ? r - p.n_heads - p.c.n_kv : r - p.n_heads;
-          dst = is_v ? static_cast<T*>(p.c.v) + page * p.c.v_page + h * p.c.v_head + in_page * p.c.v_slot
-                     : static_cast<T*>(p.c.k) + page * p.c.k_page + h * p.c.k_head + in_page * p.c.k_slot;
+          put(is_v ? static_cast<T*>(p.c.v) + page * p.c.v_page + h * p.c.v_head + in_page * p.c.v_slot
+                   : static_cast<T*>(p.c.k) + page * p.c.k_page + h * p.c.k_head + in_page * p.c.k_slot, y);
         }
-        if (dst) *reinterpret_cast<uint4*>(dst + sub * 8) = y;
       }
     }
     load(row0 + UNROLL * per_tok);

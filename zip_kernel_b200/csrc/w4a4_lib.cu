@@ -98,10 +98,14 @@ cudaError_t set_kernel_attributes() {
   set(pp::prefill_pair_gemm_kernel<true, true, true>, pp::smem_bytes(true));
   set(wide::prefill_wide_gemm_kernel<false>, wide::smem_bytes());
   set(wide::prefill_wide_gemm_kernel<true>, wide::smem_bytes());
-  set(csum::cache_sums_kernel<__half, 64>, csum::smem_bytes<64>());
-  set(csum::cache_sums_kernel<__half, 128>, csum::smem_bytes<128>());
-  set(csum::cache_sums_kernel<__nv_bfloat16, 64>, csum::smem_bytes<64>());
-  set(csum::cache_sums_kernel<__nv_bfloat16, 128>, csum::smem_bytes<128>());
+  set(csum::cache_sums_kernel<__half, 64, csum::NARROW>, csum::smem_bytes<64, csum::NARROW>());
+  set(csum::cache_sums_kernel<__half, 64, csum::MAX_COLS>, csum::smem_bytes<64, csum::MAX_COLS>());
+  set(csum::cache_sums_kernel<__half, 128, csum::NARROW>, csum::smem_bytes<128, csum::NARROW>());
+  set(csum::cache_sums_kernel<__half, 128, csum::MAX_COLS>, csum::smem_bytes<128, csum::MAX_COLS>());
+  set(csum::cache_sums_kernel<__nv_bfloat16, 64, csum::NARROW>, csum::smem_bytes<64, csum::NARROW>());
+  set(csum::cache_sums_kernel<__nv_bfloat16, 64, csum::MAX_COLS>, csum::smem_bytes<64, csum::MAX_COLS>());
+  set(csum::cache_sums_kernel<__nv_bfloat16, 128, csum::NARROW>, csum::smem_bytes<128, csum::NARROW>());
+  set(csum::cache_sums_kernel<__nv_bfloat16, 128, csum::MAX_COLS>, csum::smem_bytes<128, csum::MAX_COLS>());
   set(ppre::paged_prefill_kernel<__half, 64>, ppre::smem_bytes<64>());
   set(ppre::paged_prefill_kernel<__half, 128>, ppre::smem_bytes<128>());
   set(ppre::paged_prefill_kernel<__nv_bfloat16, 64>, ppre::smem_bytes<64>());

@@ -18,7 +18,6 @@ No counterpart in the reference, whose layer harness uses PyTorch here (bench/la
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -81,45 +80,68 @@ class PagedKV:
             block_table.data_ptr(), max(ts[0], self.max_pages), self.n_pages, self.page_size, self.n_kv_heads, self.head_dim,
             self.n_seqs, self.max_pages, DTYPES[self.dtype])
         self._ptr = ctypes.addressof(self._arg)
+        self._cu_shape, self._len_shape = (self.n_seqs + 1,), (self.n_seqs,)
+        self._sums_shape = (self.n_seqs, self.n_kv_heads, self.max_slots)
+        self._scale = self.head_dim ** -0.5
 
+
+# The checks below run on every call of a decode loop, whose kernels take a few microseconds: each attribute of a tensor is
+# asked for once (a shape or a stride costs a third of a microsecond).
 
 def _check_seqs(kv: PagedKV, cu_seqlens, lengths):
-    if cu_seqlens.dtype is not torch.int32 or cu_seqlens.shape != (kv.n_seqs + 1,) or not cu_seqlens.is_contiguous():
-        raise ValueError(f"cu_seqlens must be contiguous int32 of {kv.n_seqs + 1} entries, got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
+    if cu_seqlens.dtype is not torch.int32 or cu_seqlens.shape != kv._cu_shape or not cu_seqlens.is_contiguous() or cu_seqlens.device != kv.device:
+        raise ValueError(f"cu_seqlens must be contiguous int32 of {kv.n_seqs + 1} entries on {kv.device}, got {cu_seqlens.dtype} "
+                         f"{tuple(cu_seqlens.shape)} on {cu_seqlens.device}")
     _check_lengths(kv, lengths)
-    if cu_seqlens.device != kv.device:
-        raise ValueError(f"cu_seqlens must be on {kv.device}, got {cu_seqlens.device}")
 
 
 def _check_lengths(kv: PagedKV, lengths):
-    if lengths.dtype is not torch.int32 or lengths.shape != (kv.n_seqs,) or not lengths.is_contiguous() or lengths.device != kv.device:
+    if lengths.dtype is not torch.int32 or lengths.shape != kv._len_shape or not lengths.is_contiguous() or lengths.device != kv.device:
         raise ValueError(f"lengths must be contiguous int32 of {kv.n_seqs} entries on {kv.device}, got {lengths.dtype} "
                          f"{tuple(lengths.shape)} on {lengths.device}")
 
 
-def _check_rows(kv: PagedKV, name: str, t: torch.Tensor):
-    if t.dtype is not kv.dtype or t.dim() != 3 or t.shape[2] != kv.head_dim or t.device != kv.device:
-        raise ValueError(f"{name} must be (T, n_heads, {kv.head_dim}) {kv.dtype} on {kv.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if t.shape[1] < 1 or t.shape[1] % kv.n_kv_heads:
-        raise ValueError(f"{name}: {t.shape[1]} heads are no multiple of the {kv.n_kv_heads} key/value heads")
+def _row_strides(shape, strides, dim):
+    """(token, head) strides, those of dimensions of one entry as if contiguous."""
+    return (strides[0] if shape[0] > 1 else shape[1] * dim), (strides[1] if shape[1] > 1 else dim)
 
 
-def _rows_ok(t: torch.Tensor) -> bool:
-    a, b, c = t.stride()
-    return (c == 1 and (t.shape[1] == 1 or (b >= t.shape[2] and b % 8 == 0)) and (t.shape[0] <= 1 or (a >= t.shape[2] and a % 8 == 0))
-            and t.data_ptr() % 16 == 0)
+def _rows_ok(tok: int, head: int, inner: int, dim: int, ptr: int) -> bool:
+    return inner == 1 and head >= dim and tok >= dim and not (tok | head) & 7 and not ptr & 15
 
 
-def _row_strides(t: torch.Tensor):
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]), (t.stride(1) if t.shape[1] > 1 else t.shape[2])
+def _query_rows(kv: PagedKV, q: torch.Tensor):
+    """(q or a copy a kernel can read, T, n_heads, token stride, head stride)"""
+    shape = q.shape
+    if q.dtype is not kv.dtype or len(shape) != 3 or shape[2] != kv.head_dim or q.device != kv.device:
+        raise ValueError(f"q must be (T, n_heads, {kv.head_dim}) {kv.dtype} on {kv.device}, got {q.dtype} {tuple(shape)} on {q.device}")
+    T, n_heads, dim = shape
+    if n_heads < 1 or n_heads % kv.n_kv_heads:
+        raise ValueError(f"q: {n_heads} heads are no multiple of the {kv.n_kv_heads} key/value heads")
+    strides = q.stride()
+    tok, head = _row_strides(shape, strides, dim)
+    if not _rows_ok(tok, head, strides[2], dim, q.data_ptr()):
+        q, tok, head = q.clone(memory_format=torch.contiguous_format), n_heads * dim, dim
+    return q, T, n_heads, tok, head
 
 
-def _out_rows(kv: PagedKV, out: Optional[torch.Tensor], T: int, n_heads: int) -> torch.Tensor:
+def _out_rows(kv: PagedKV, out: Optional[torch.Tensor], T: int, n_heads: int):
+    """(output, token stride, head stride)"""
+    dim = kv.head_dim
     if out is None:
-        return torch.empty((T, n_heads, kv.head_dim), dtype=kv.dtype, device=kv.device)
-    if out.shape != (T, n_heads, kv.head_dim) or out.dtype is not kv.dtype or out.device != kv.device or not _rows_ok(out):
-        raise ValueError(f"out must be ({T}, {n_heads}, {kv.head_dim}) {kv.dtype} on {kv.device} with contiguous rows over 16-byte strides")
-    return out
+        return torch.empty((T, n_heads, dim), dtype=kv.dtype, device=kv.device), n_heads * dim, dim
+    shape, strides = out.shape, out.stride()
+    if shape == (T, n_heads, dim) and out.dtype is kv.dtype and out.device == kv.device:
+        tok, head = _row_strides(shape, strides, dim)
+        if _rows_ok(tok, head, strides[2], dim, out.data_ptr()):
+            return out, tok, head
+    raise ValueError(f"out must be ({T}, {n_heads}, {dim}) {kv.dtype} on {kv.device} with contiguous rows over 16-byte strides, got "
+                     f"{out.dtype} {tuple(shape)} with strides {tuple(strides)} on {out.device}")
+
+
+def _aligned(t: Optional[torch.Tensor]):
+    """Contiguous and on a 16-byte boundary, copied where it is not."""
+    return t if t is None or (t.is_contiguous() and not t.data_ptr() & 15) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _max_q(max_q_len: Optional[int], T: int) -> int:
@@ -128,6 +150,15 @@ def _max_q(max_q_len: Optional[int], T: int) -> int:
     if max_q_len < 0:
         raise ValueError(f"max_q_len must not be negative, got {max_q_len}")
     return min(int(max_q_len), T)
+
+
+def _check_scale(kv: PagedKV, scale: Optional[float]) -> float:
+    if scale is None:
+        return kv._scale
+    scale = float(scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return scale
 
 
 @traced("cuda.qkv_rope_cache")
@@ -143,38 +174,43 @@ def qkv_rope_cache_cuda(qkv: torch.Tensor, kv: PagedKV, cu_seqlens: torch.Tensor
     that is given: the number of slots evicted from the sequence.  ``interleaved``: pairs are neighbours, else ``i`` and
     ``i + rot_dim / 2``.  Everything is computed in float32 and rounded once.  Tokens behind the last sequence are left as
     ``out`` holds them (undefined without ``out``); ``out`` may be the query columns of ``qkv``."""
-    if qkv.dim() != 2 or qkv.dtype is not kv.dtype or qkv.device != kv.device:
-        raise ValueError(f"qkv must be 2-D {kv.dtype} on {kv.device}, got {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}")
-    T, width, D = int(qkv.shape[0]), int(qkv.shape[1]), kv.head_dim
+    shape, D, device, dtype = qkv.shape, kv.head_dim, kv.device, kv.dtype
+    if len(shape) != 2 or qkv.dtype is not dtype or qkv.device != device:
+        raise ValueError(f"qkv must be 2-D {dtype} on {device}, got {qkv.dtype} {tuple(shape)} on {qkv.device}")
+    T, width = shape
     n_heads = width // D - 2 * kv.n_kv_heads
     if width % D or n_heads < 1 or n_heads % kv.n_kv_heads:
         raise ValueError(f"qkv of width {width} is not n_heads + 2 * {kv.n_kv_heads} heads of {D}, n_heads a multiple of {kv.n_kv_heads}")
     _check_seqs(kv, cu_seqlens, lengths)
-    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2 or cos.shape != sin.shape:
+    table = cos.shape
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(table) != 2 or sin.shape != table:
         raise ValueError("cos and sin must be float32 of one shape (max_pos, rot_dim / 2)")
-    if cos.device != kv.device or sin.device != kv.device:
-        raise ValueError(f"cos and sin must be on {kv.device}")
-    rot = 2 * int(cos.shape[1])
-    if rot % 16 or rot > D:
-        raise ValueError(f"the rotated width must be a multiple of 16 up to {D}, got {rot}")
+    if cos.device != device or sin.device != device:
+        raise ValueError(f"cos and sin must be on {device}")
+    max_pos, half = table
+    if half % 8 or 2 * half > D:
+        raise ValueError(f"the rotated width must be a multiple of 16 up to {D}, got {2 * half}")
     for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None and (w.shape != (D,) or w.dtype is not kv.dtype or w.device != kv.device):
-            raise ValueError(f"{name} must be ({D},) {kv.dtype} on {kv.device}")
+        if w is not None and (w.shape != (D,) or w.dtype is not dtype or w.device != device):
+            raise ValueError(f"{name} must be ({D},) {dtype} on {device}")
     if offsets is not None:
         _check_lengths(kv, offsets)
-    q = _out_rows(kv, out, T, n_heads)
+    q, tok, head = _out_rows(kv, out, T, n_heads)
     if T == 0 or kv.n_seqs == 0:
         return q
-    if qkv.stride(1) != 1 or (T > 1 and (qkv.stride(0) < width or qkv.stride(0) % 8)) or qkv.data_ptr() % 16:
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
-    cos, sin, q_norm, k_norm = (None if t is None else t if t.is_contiguous() and t.data_ptr() % 16 == 0
-                                else t.clone(memory_format=torch.contiguous_format) for t in (cos, sin, q_norm, k_norm))
-    tok, head = _row_strides(q)
-    with _lib.on_device(kv.device):
-        _lib.check(_L.w4a4_qkv_rope_cache(
-            kv._ptr, qkv.data_ptr(), qkv.stride(0) if T > 1 else width, cu_seqlens.data_ptr(), lengths.data_ptr(), cos.data_ptr(),
-            sin.data_ptr(), int(cos.shape[0]), rot, _lib.ptr(q_norm), _lib.ptr(k_norm), float(eps), int(interleaved),
-            _lib.ptr(offsets), q.data_ptr(), tok, head, T, n_heads, _lib.stream_ptr(kv.device)), "qkv_rope_cache")
+    ld, inner = qkv.stride()
+    if T == 1:
+        ld = width
+    if inner != 1 or ld < width or ld & 7 or qkv.data_ptr() & 15:
+        qkv, ld = qkv.clone(memory_format=torch.contiguous_format), width
+    cos, sin, q_norm, k_norm = _aligned(cos), _aligned(sin), _aligned(q_norm), _aligned(k_norm)
+    with _lib.on_device(device):
+        status = _L.w4a4_qkv_rope_cache(
+            kv._ptr, qkv.data_ptr(), ld, cu_seqlens.data_ptr(), lengths.data_ptr(), cos.data_ptr(), sin.data_ptr(), max_pos, 2 * half,
+            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps, interleaved,
+            None if offsets is None else offsets.data_ptr(), q.data_ptr(), tok, head, T, n_heads, _lib.stream_ptr(device))
+    if status:
+        _lib.check(status, "qkv_rope_cache")
     return q
 
 
@@ -190,33 +226,34 @@ def paged_attention_cuda(q: torch.Tensor, kv: PagedKV, cu_seqlens: torch.Tensor,
     default); pass 1 for a decode step, so that only the kernel for few rows is launched.  A row that sees no slot is
     zero, its ``lse`` minus infinity.  Tokens behind the last sequence are left as ``out`` holds them (undefined without
     ``out``, like their ``lse``).  Values within a sequence's length must be finite; what lies behind it does not matter."""
-    _check_rows(kv, "q", q)
+    q, T, n_heads, tok, head = _query_rows(kv, q)
     _check_seqs(kv, cu_seqlens, lengths)
-    T, n_heads = int(q.shape[0]), int(q.shape[1])
-    o = _out_rows(kv, out, T, n_heads)
+    scale = _check_scale(kv, scale)
+    o, o_tok, o_head = _out_rows(kv, out, T, n_heads)
     lse = torch.empty((T, n_heads), dtype=torch.float32, device=kv.device) if return_lse else None
     max_q = _max_q(max_q_len, T)
     if T and kv.n_seqs and max_q:
-        if not _rows_ok(q):
-            q = q.clone(memory_format=torch.contiguous_format)
-        (qt, qh), (ot, oh) = _row_strides(q), _row_strides(o)
-        with _lib.on_device(kv.device):
-            ws = _lib.attention_workspace(kv, T, n_heads, max_q)
-            _lib.check(_L.w4a4_paged_attention(
-                kv._ptr, q.data_ptr(), qt, qh, cu_seqlens.data_ptr(), lengths.data_ptr(), o.data_ptr(), ot, oh, _lib.ptr(lse),
-                T, n_heads, max_q, kv.head_dim ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel(),
-                _lib.stream_ptr(kv.device)), "paged_attention")
+        device = kv.device
+        with _lib.on_device(device):
+            stream = _lib.stream_ptr(device)
+            ws = _lib.attention_workspace(kv, T, n_heads, max_q, stream)
+            status = _L.w4a4_paged_attention(
+                kv._ptr, q.data_ptr(), tok, head, cu_seqlens.data_ptr(), lengths.data_ptr(), o.data_ptr(), o_tok, o_head,
+                None if lse is None else lse.data_ptr(), T, n_heads, max_q, scale, ws.data_ptr(), ws.numel(), stream)
+        if status:
+            _lib.check(status, "paged_attention")
     return (o, lse) if return_lse else o
 
 
 def _check_sums(kv: PagedKV, sums):
-    if sums.dtype is not torch.float32 or sums.shape != (kv.n_seqs, kv.n_kv_heads, kv.max_slots) or sums.device != kv.device:
-        raise ValueError(f"sums must be float32 ({kv.n_seqs}, {kv.n_kv_heads}, {kv.max_slots}) on {kv.device}, got {sums.dtype} "
-                         f"{tuple(sums.shape)} on {sums.device}")
-    st = _strides(sums)
-    if (sums.shape[2] > 1 and st[2] != 1) or (sums.shape[1] > 1 and st[1] < kv.max_slots) or (sums.shape[0] > 1 and st[0] < kv.max_slots):
+    """(sequence stride, head stride)"""
+    shape, slots = sums.shape, kv.max_slots
+    if sums.dtype is not torch.float32 or shape != kv._sums_shape or sums.device != kv.device:
+        raise ValueError(f"sums must be float32 {kv._sums_shape} on {kv.device}, got {sums.dtype} {tuple(shape)} on {sums.device}")
+    seq, head, inner = _strides(sums)
+    if (shape[2] > 1 and inner != 1) or (shape[1] > 1 and head < slots) or (shape[0] > 1 and seq < slots):
         raise ValueError(f"the rows of sums must be contiguous and apart, got strides {tuple(sums.stride())}")
-    return max(st[0], kv.max_slots), max(st[1], kv.max_slots)
+    return max(seq, slots), max(head, slots)
 
 
 @traced("cuda.cache_weight_sums")
@@ -228,25 +265,24 @@ def cache_weight_sums_cuda(q: torch.Tensor, kv: PagedKV, cu_seqlens: torch.Tenso
     same queries and lengths.  The heads that share a key/value head are added up.  Slots behind a sequence's length are
     left as they are.  To count the last tokens of a chunk only, pass their rows of ``q`` and ``lse`` and their
     ``cu_seqlens``."""
-    _check_rows(kv, "q", q)
+    q, T, n_heads, tok, head = _query_rows(kv, q)
     _check_seqs(kv, cu_seqlens, lengths)
-    T, n_heads = int(q.shape[0]), int(q.shape[1])
     if lse.shape != (T, n_heads) or lse.dtype is not torch.float32 or lse.device != kv.device:
         raise ValueError(f"lse must be float32 ({T}, {n_heads}) on {kv.device}, got {lse.dtype} {tuple(lse.shape)} on {lse.device}")
+    scale = _check_scale(kv, scale)
     if sums is None:
-        sums = torch.zeros((kv.n_seqs, kv.n_kv_heads, kv.max_slots), dtype=torch.float32, device=kv.device)
-    seq, head = _check_sums(kv, sums)
+        sums = torch.zeros(kv._sums_shape, dtype=torch.float32, device=kv.device)
+    seq, group = _check_sums(kv, sums)
     max_q = _max_q(max_q_len, T)
     if T and kv.n_seqs and max_q:
-        if not _rows_ok(q):
-            q = q.clone(memory_format=torch.contiguous_format)
         lse = lse.contiguous()
-        qt, qh = _row_strides(q)
-        with _lib.on_device(kv.device):
-            _lib.check(_L.w4a4_cache_weight_sums(
-                kv._ptr, q.data_ptr(), qt, qh, cu_seqlens.data_ptr(), lengths.data_ptr(), lse.data_ptr(), sums.data_ptr(), seq, head,
-                T, n_heads, max_q, kv.head_dim ** -0.5 if scale is None else float(scale), _lib.stream_ptr(kv.device)),
-                "cache_weight_sums")
+        device = kv.device
+        with _lib.on_device(device):
+            status = _L.w4a4_cache_weight_sums(
+                kv._ptr, q.data_ptr(), tok, head, cu_seqlens.data_ptr(), lengths.data_ptr(), lse.data_ptr(), sums.data_ptr(), seq, group,
+                T, n_heads, max_q, scale, _lib.stream_ptr(device))
+        if status:
+            _lib.check(status, "cache_weight_sums")
     return sums
 
 
@@ -277,9 +313,11 @@ def cache_evict_cuda(kv: PagedKV, lengths: torch.Tensor, sums: torch.Tensor, bud
     new_sums = torch.empty((kv.n_seqs, kv.n_kv_heads, into.max_slots), dtype=torch.float32, device=kv.device)
     if kv.n_seqs:
         with _lib.on_device(kv.device):
-            _lib.check(_L.w4a4_cache_evict(
+            status = _L.w4a4_cache_evict(
                 kv._ptr, into._ptr, lengths.data_ptr(), sums.data_ptr(), seq, head, budget, n_sink, n_recent, kept.data_ptr(),
-                new_lengths.data_ptr(), new_sums.data_ptr(), _lib.stream_ptr(kv.device)), "cache_evict")
+                new_lengths.data_ptr(), new_sums.data_ptr(), _lib.stream_ptr(kv.device))
+        if status:
+            _lib.check(status, "cache_evict")
     return kept, new_lengths, new_sums
 
 
