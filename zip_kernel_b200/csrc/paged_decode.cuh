@@ -12,7 +12,7 @@
 // is joined by the CTA that finishes its last part (the parts' order, and so the result's bits, depend on the lengths
 // alone).
 //
-// A CTA is one warp that issues copies (TMA boxes of one page each, 128-byte swizzle, a ring of tiles) and two teams of
+// A CTA has one warp that issues copies (TMA boxes of one page each, 128-byte swizzle, a ring of tiles) and two teams of
 // four that compute on alternate tiles, each warp on 16 slots of a tile with a maximum, sum and output of its own, joined
 // at the end of a unit: no barrier between the warps inside a unit.  One team alone takes about 2000 clocks from a
 // tile's arrival to handing its place back, more than the tile takes to arrive (4.3 TB/s over 148 SMs).
@@ -33,7 +33,11 @@ using namespace kv;
 
 constexpr int TILE = 64, WK = 16, ROWS = 16;
 constexpr int SHARE = TILE / WK, TEAMS = 2, WARPS = TEAMS * SHARE;      // warps that share a tile, teams that take turns
-constexpr int THREADS = (WARPS + 1) * 32;
+constexpr int THREADS = (WARPS + 4) * 32;                    // a third warpgroup: the copying warp, and three to fill it
+// Registers of the launch, 168 a thread, dealt out again: with 168 for the arithmetic the loop over tiles spills (a
+// batch of 32 histories up to 4096 slots 72 us with 208 bytes spilled, 57 us with 116).
+constexpr int REG_COPY = 72, REG_COMPUTE = 216;
+static_assert(REG_COPY + 2 * REG_COMPUTE <= 3 * 168, "the warpgroups share the registers of the launch");
 constexpr int MAX_RUNS = 256;                                // CTAs of a launch
 
 enum : int { SITE_PDEC_FULL = 35, SITE_PDEC_EMPTY, SITE_PDEC_DRAIN };
@@ -50,8 +54,7 @@ struct Layout {
   // a part of a unit in the workspace: m and l of the rows, then their outputs
   static constexpr int PART = ROWS * (2 + DIM);
   static constexpr int joined = STAGES * STAGE;              // float [SHARE][ROWS][DIM]; weights of the parts of a unit
-  static constexpr int JOINED = MAX_RUNS * ROWS * 8;
-  static_assert(SHARE * ROWS * DIM * 4 <= JOINED, "the outputs of a team fit");
+  static constexpr int JOINED = SHARE * ROWS * DIM * 4 > MAX_RUNS * ROWS * 4 ? SHARE * ROWS * DIM * 4 : MAX_RUNS * ROWS * 4;
   static constexpr int ml = joined + JOINED;                 // float [SHARE][ROWS][2]
   static constexpr int bars = ml + SHARE * ROWS * 2 * 4;
   static constexpr int total = bars + 2 * STAGES * 8 + 16;
@@ -111,6 +114,65 @@ __device__ __forceinline__ void ldmatrix_x4_t(uint32_t (&r)[4], uint32_t a) {
 }
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
 
+// Two elements of a row's output (a row that sees nothing is zero), and its lse with the first.
+template <typename T>
+__device__ __forceinline__ void write_out(const Params& p, int tok, int hd, int d, const float2& acc, float m, float l) {
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)tok * p.o_tok + (long long)hd * p.o_head + d) = pack2<T>(acc.x * inv, acc.y * inv);
+  if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = l > 0.f ? (m + log2f(l)) * LN2 : l == l ? neg_inf() : l;
+}
+
+// Joins the parts of a unit (all computing warps).
+template <typename T, int DIM>
+__device__ __forceinline__ void join_parts(const Params& p, long long c0, int parts, int rows, int q0, int head, int row0, float* wt, float* ml) {
+  using L = Layout<DIM>;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the first part is the second of its run's two (the unit begins in that run), the others their run's first
+  auto part_of = [&](int k) { return p.parts + (2 * (c0 + k) + (k == 0 ? 1 : 0)) * L::PART; };
+  // the outputs of the first parts are on their way while the weights (wt [row][part]) are made
+  constexpr int AHEAD = 16;
+  const int elements = rows * (DIM / 2);
+  float2 v[AHEAD];
+  auto fetch = [&](int e, int k0) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (e < elements && k0 + k < parts)
+        v[k] = __ldcg(reinterpret_cast<const float2*>(part_of(k0 + k) + 2 * ROWS + e / (DIM / 2) * DIM + (e % (DIM / 2)) * 2));
+  };
+  fetch(tid, 0);
+  for (int r = warp; r < rows; r += WARPS) {
+    float mx = neg_inf(), lt = 0.f;
+    for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, __ldcg(part_of(k) + 2 * r));
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+    for (int k = lane; k < parts; k += 32) {
+      const float2 x = __ldcg(reinterpret_cast<const float2*>(part_of(k)) + r);
+      const float a = x.x == neg_inf() ? (x.y == x.y ? 0.f : 1.f) : ex2(x.x - mx);
+      lt += a * x.y;
+      wt[r * MAX_RUNS + k] = a;
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) lt += __shfl_xor_sync(0xffffffffu, lt, s);
+    if (lane == 0) { ml[2 * r] = mx; ml[2 * r + 1] = lt; }
+  }
+  compute_barrier();
+  for (int e = tid; e < elements; e += WARPS * 32) {
+    const int r = e / (DIM / 2), d = (e % (DIM / 2)) * 2;
+    float2 acc = make_float2(0.f, 0.f);
+    for (int k0 = 0; k0 < parts; k0 += AHEAD) {
+      if (e != tid || k0 > 0) fetch(e, k0);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (k0 + k < parts) {
+          const float a = wt[r * MAX_RUNS + k0 + k];
+          acc.x += a * v[k].x;
+          acc.y += a * v[k].y;
+        }
+    }
+    write_out<T>(p, q0 + (row0 + r) / p.group, head * p.group + (row0 + r) % p.group, d, acc, ml[2 * r], ml[2 * r + 1]);
+  }
+}
+
 // MH: eight-row halves of a row tile that are in use
 template <typename T, int DIM, int MH>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -144,7 +206,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   const uint32_t ring = smem_u32(sm);
   bool ok = true;                                            // no wait of this thread has given up
 
-  if (warp == WARPS) {
+  if (warp >= WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_COPY));
+    if (warp == WARPS) {
     // ------------------------------------------------------------ copies
     Walk<Params> w;
     w.start(p, begin);
@@ -178,7 +242,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       if (w.at - w.tile + stop >= end) break;
       w.next_unit(p);
     }
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_COMPUTE));
     // ------------------------------------------------------------ arithmetic
     const int g = lane >> 2, c2 = (lane & 3) * 2;            // fragment row (and row + 8), first of two columns
     Walk<Params> w;
@@ -363,8 +429,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       // (after a wait that gave up the warp still goes to every barrier that the others wait at)
       compute_barrier();
       const bool whole = first == 0 && stop == u.tiles - PAD;
-      auto w_tok = [&](int r) { return u.q.q0 + (row0 + r) / p.group; };
-      auto w_head = [&](int r) { return u.head * p.group + (row0 + r) % p.group; };
       const long long u0 = u.unit_first() + PAD, u1 = u0 + u.tiles - PAD;
       float* part = p.parts + (2 * c + (u0 < begin ? 0 : 1)) * L::PART;
       for (int e = tid; e < rows * (DIM / 2); e += WARPS * 32) {
@@ -382,10 +446,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           acc.y += a * v.y;
         }
         if (whole) {
-          const int tok = w_tok(r), hd = w_head(r);
-          const float inv = lt > 0.f ? 1.f / lt : 0.f;       // a row that sees nothing is zero
-          *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)tok * p.o_tok + (long long)hd * p.o_head + d) = pack2<T>(acc.x * inv, acc.y * inv);
-          if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = lt > 0.f ? (mx + log2f(lt)) * LN2 : lt == lt ? neg_inf() : lt;
+          write_out<T>(p, u.q.q0 + (row0 + r) / p.group, u.head * p.group + (row0 + r) % p.group, d, acc, mx, lt);
         } else {
           *reinterpret_cast<float2*>(part + 2 * ROWS + r * DIM + d) = acc;
           if (d == 0) { part[2 * r] = mx; part[2 * r + 1] = lt; }
@@ -394,9 +455,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       if (!whole) {
         // runs the unit falls into: run(x) = the c with c * total / runs <= x < (c + 1) * total / runs
         const long long c0 = ((u0 + 1) * runs - 1) / total, c1 = (u1 * runs - 1) / total;
-        __threadfence();
         compute_barrier();
         if (tid == 0) {
+          __threadfence();                                   // (and with it what the barrier has ordered before)
           int* a = p.arrived + c0;                           // (at most one unit is cut for the first time in a run)
           const bool last = atomicAdd(a, 1) == (int)(c1 - c0);
           if (last) *a = 0;
@@ -404,43 +465,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           *last_flag = last;
         }
         compute_barrier();
-        if (*last_flag) {
-          // the first part is the second of its run's two (the unit begins in that run), the others their run's first
-          const int parts = (int)(c1 - c0) + 1;
-          auto part_of = [&](int k) { return p.parts + (2 * (c0 + k) + (k == 0 ? 1 : 0)) * L::PART; };
-          float2* wt = reinterpret_cast<float2*>(joined);    // [parts][rows] m and l, then weight and l
-          for (int e = tid; e < parts * rows; e += WARPS * 32) wt[e] = __ldcg(reinterpret_cast<const float2*>(part_of(e / rows)) + e % rows);
-          compute_barrier();
-          if (tid < rows) {
-            float mx = neg_inf(), lt = 0.f;
-            for (int k = 0; k < parts; ++k) mx = fmaxf(mx, wt[k * rows + tid].x);
-            for (int k = 0; k < parts; ++k) {
-              float2 v = wt[k * rows + tid];
-              v.x = v.x == neg_inf() ? 0.f : ex2(v.x - mx);
-              lt += v.x * v.y;
-              wt[k * rows + tid] = v;
-            }
-            ml[2 * tid] = mx;
-            ml[2 * tid + 1] = lt;
-          }
-          compute_barrier();
-          for (int e = tid; e < rows * (DIM / 2); e += WARPS * 32) {
-            const int r = e / (DIM / 2), d = (e % (DIM / 2)) * 2;
-            float2 acc = make_float2(0.f, 0.f);
-#pragma unroll 8
-            for (int k = 0; k < parts; ++k) {
-              const float a = wt[k * rows + r].x;
-              const float2 v = __ldcg(reinterpret_cast<const float2*>(part_of(k) + 2 * ROWS + r * DIM + d));
-              acc.x += a * v.x;
-              acc.y += a * v.y;
-            }
-            const float mx = ml[2 * r], lt = ml[2 * r + 1];
-            const int tok = w_tok(r), hd = w_head(r);
-            const float inv = lt > 0.f ? 1.f / lt : 0.f;
-            *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)tok * p.o_tok + (long long)hd * p.o_head + d) = pack2<T>(acc.x * inv, acc.y * inv);
-            if (p.lse && d == 0) p.lse[(long long)tok * p.n_heads + hd] = lt > 0.f ? (mx + log2f(lt)) * LN2 : lt == lt ? neg_inf() : lt;
-          }
-        }
+        if (*last_flag) join_parts<T, DIM>(p, c0, (int)(c1 - c0) + 1, rows, u.q.q0, u.head, row0, joined, ml);
       }
       compute_barrier();                                     // the joining buffers are free again
       }
