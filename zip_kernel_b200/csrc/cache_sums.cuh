@@ -164,13 +164,10 @@ cache_sums_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   if (warp == WARP_COPY) grid_dependency_wait_for_async_reads();
   else grid_dependency_wait();
 
-  const long long total = total_tiles(p);
-  const long long runs = min((long long)gridDim.x, total), c = blockIdx.x;
   bool ok = true;                                          // no wait of this thread has given up
-  if (c < runs) {
-    const long long begin = c * total / runs, end = (c + 1) * total / runs;
-    Walk<Params> w;
-    w.start(p, begin);
+  Walk<Params> w;
+  long long total, runs, begin, end;
+  if (w.start(p, gridDim.x, blockIdx.x, total, runs, begin, end)) {
     if (warp == WARP_COPY) {
       // ---------------------------------------------------------- copies
       PagesAhead pages;

@@ -199,10 +199,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   if (warp == WARPS) grid_dependency_wait_for_async_reads();
   else grid_dependency_wait();
 
-  const long long total = total_tiles(p);
-  const long long runs = min((long long)gridDim.x, total), c = blockIdx.x;
-  if (c >= runs) return;
-  const long long begin = c * total / runs, end = (c + 1) * total / runs;
+  const int c = blockIdx.x;                                  // run; there may be fewer, then the CTA has nothing to do
   const uint32_t ring = smem_u32(sm);
   bool ok = true;                                            // no wait of this thread has given up
 
@@ -211,12 +208,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     if (warp == WARPS) {
     // ------------------------------------------------------------ copies
     Walk<Params> w;
-    w.start(p, begin);
+    long long total, runs, begin, end;
+    const bool any = w.start(p, gridDim.x, c, total, runs, begin, end);
     PagesAhead pages;
     int s = 0;
     uint32_t ph = 1;
     long long n = 0;
-    while (ok) {
+    while (any && ok) {
       const int stop = (int)min((long long)w.tiles, w.tile + (end - w.at));
       for (int t = max(w.tile - PAD, 0); t < stop - PAD; ++t, ++n) {
         if (n >= L::STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph, SITE_PDEC_EMPTY));
@@ -248,7 +246,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     // ------------------------------------------------------------ arithmetic
     const int g = lane >> 2, c2 = (lane & 3) * 2;            // fragment row (and row + 8), first of two columns
     Walk<Params> w;
-    w.start(p, begin);
+    long long total, runs, begin, end;
+    const bool any = w.start(p, gridDim.x, c, total, runs, begin, end);
     const int team = warp / SHARE, share = warp % SHARE;
     uint32_t n = 0;                                          // tiles of the run before this unit
     // addresses inside a tile: this lane's ldmatrix row and the swizzle of its 16-byte chunks
@@ -272,8 +271,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
       }
     };
-    load_rows(w);
-    while (true) {
+    if (any) load_rows(w);
+    while (any) {
       const int row0 = w.row_tile * ROWS, rows = min(ROWS, w.q.q_len * p.group - row0);
       float o[DIM / 8][2 * MH], m[MH], l[MH];
 #pragma unroll

@@ -74,35 +74,77 @@ struct Walk {
     q = load_seq(p.s, b);
     unit_shape(p, q, row_tiles, tiles);
   }
-  // whole warp; x below the total
-  __device__ __forceinline__ void start(const Params& p, long long x) {
+  // Whole warp: all tiles of the call, run c of min(grid, total), and this walk at its first tile; false when there is
+  // no such run.  The first 32 sequences are read once for both.
+  __device__ __forceinline__ bool start(const Params& p, int grid, int c, long long& total, long long& runs, long long& begin, long long& end) {
     const int lane = threadIdx.x & 31;
-    long long tiles_before = 0;
-    for (int base = 0; base < p.s.n; base += 32) {
+    Seq first{};
+    int rt0 = 0, n0 = 0;
+    if (lane < p.s.n) {
+      first = load_seq(p.s, lane);
+      unit_shape(p, first, rt0, n0);
+    }
+    long long w0 = (long long)rt0 * n0 * p.c.n_kv;
+    scan(w0);
+    total = 0;
+    for (int i = 32 + lane; i < p.s.n; i += 32) {
+      int rt, n;
+      unit_shape(p, load_seq(p.s, i), rt, n);
+      total += (long long)rt * n * p.c.n_kv;
+    }
+    if (p.s.n > 32)
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const long long head0 = __shfl_sync(0xffffffffu, w0, 31);
+    total += head0;
+    runs = min((long long)grid, total);
+    if (c >= runs) return false;
+    begin = c * total / runs;
+    end = (c + 1) * total / runs;
+    at = begin;
+    if (begin < head0) {
+      const int i = __ffs(__ballot_sync(0xffffffffu, w0 > begin)) - 1;
+      const long long before = __shfl_sync(0xffffffffu, w0, (i - 1) & 31);
+      b = i;
+      q.q0 = __shfl_sync(0xffffffffu, first.q0, i);
+      q.q_len = __shfl_sync(0xffffffffu, first.q_len, i);
+      q.len = __shfl_sync(0xffffffffu, first.len, i);
+      unit_shape(p, q, row_tiles, tiles);
+      inside(begin - (i ? before : 0));
+      return true;
+    }
+    long long before = head0;
+    for (int base = 32; base < p.s.n; base += 32) {
       int rt = 0, n = 0;
       if (base + lane < p.s.n) unit_shape(p, load_seq(p.s, base + lane), rt, n);
       long long w = (long long)rt * n * p.c.n_kv;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const long long a = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += a;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, tiles_before + w > x);
+      scan(w);
+      const unsigned past = __ballot_sync(0xffffffffu, before + w > begin);
       if (past) {
         const int i = __ffs(past) - 1;
         const long long w1 = __shfl_sync(0xffffffffu, w, (i - 1) & 31);
-        tiles_before += i ? w1 : 0;
         set_seq(p, base + i);
-        const long long rem = x - tiles_before, per_head = (long long)row_tiles * tiles;
-        head = (int)(rem / per_head);
-        const long long r2 = rem - head * per_head;
-        row_tile = (int)(r2 / tiles);
-        tile = (int)(r2 - (long long)row_tile * tiles);
-        at = x;
-        return;
+        inside(begin - before - (i ? w1 : 0));
+        return true;
       }
-      tiles_before += __shfl_sync(0xffffffffu, w, 31);
+      before += __shfl_sync(0xffffffffu, w, 31);
     }
+    return false;                                            // (not reached: begin is below the total)
+  }
+  __device__ __forceinline__ static void scan(long long& w) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const long long a = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += a;
+    }
+  }
+  __device__ __forceinline__ void inside(long long rem) {
+    const long long per_head = (long long)row_tiles * tiles;
+    head = (int)(rem / per_head);
+    const long long r2 = rem - head * per_head;
+    row_tile = (int)(r2 / tiles);
+    tile = (int)(r2 - (long long)row_tile * tiles);
   }
   // to the first tile of the next unit (there is one)
   __device__ __forceinline__ void next_unit(const Params& p) {
@@ -116,20 +158,6 @@ struct Walk {
   }
   __device__ __forceinline__ long long unit_first() const { return at - tile; }
 };
-
-// All tiles of the call (whole warp).
-template <typename Params>
-__device__ __forceinline__ long long total_tiles(const Params& p) {
-  long long w = 0;
-  for (int b = threadIdx.x & 31; b < p.s.n; b += 32) {
-    int rt, n;
-    unit_shape(p, load_seq(p.s, b), rt, n);
-    w += (long long)rt * n * p.c.n_kv;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) w += __shfl_xor_sync(0xffffffffu, w, o);
-  return w;
-}
 
 // Page numbers of a sequence's copy boxes (`box` slots each, none crosses a page), 32 at a time in the lanes of the warp
 // that issues the copies, and the next 32 already asked for: a look-up per tile would put a load's latency, longer than a
