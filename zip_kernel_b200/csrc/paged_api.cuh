@@ -122,7 +122,7 @@ struct AttnPlan {
   bool few, many;             // the kernel for few rows, the one for many
   int few_rows;               // a sequence with at most this many rows goes to the former
   int toks;                   // tokens of a row tile of the latter
-  size_t few_parts, many_parts, total;
+  size_t few_parts, many_parts, joins, total;
 };
 // A sequence with up to this many rows (new tokens x heads of a group) goes to the kernel for few rows: one row tile of it.
 constexpr int ATTN_FEW_ROWS = pdec::ROWS;
@@ -134,12 +134,13 @@ AttnPlan attn_plan(const w4a4_paged_kv* c, int T, int n_heads, int max_q, int sm
   a.few = !a.many || c->n_seqs > 1;                        // one sequence: whatever its length, one kernel
   a.few_rows = !a.many ? 0x7fffffff : a.few ? ATTN_FEW_ROWS : 0;
   a.toks = a.many ? ppre::ROWS / group : 0;
-  // (the counters are shared: the kernels of a call run one after the other and leave them zero)
   size_t off = W4A4_ATTENTION_STATE_BYTES;
   a.few_parts = off;
   if (a.few) off += round_up((size_t)2 * sm_count * (c->head_dim == 128 ? pdec::Layout<128>::PART : pdec::Layout<64>::PART) * 4, 256);
   a.many_parts = off;
   if (a.many) off += (size_t)2 * sm_count * (c->head_dim == 128 ? ppre::Layout<128>::PART : ppre::Layout<64>::PART) * 4;
+  a.joins = off;
+  if (a.many) off += (size_t)sm_count * sizeof(ppre::Join);
   a.total = off;
   return a;
 }
@@ -280,8 +281,8 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
     p.o_tok = out_tok_stride;
     p.o_head = out_head_stride;
     p.lse = lse;
-    p.arrived = reinterpret_cast<int*>(ws);
     p.parts = reinterpret_cast<float*>(ws + plan.many_parts);
+    p.joins = ws + plan.joins;
     p.n_heads = n_heads;
     p.group = group;
     p.box = box_slots(cache->page_size, ppre::TILE);
@@ -298,6 +299,10 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
     cudaError_t e = launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(ppre::THREADS),
                               d128 ? ppre::smem_bytes<128>() : ppre::smem_bytes<64>(), st, 1, tk, tv, tq, p);
     if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "prompt attention kernel launch: %s", cudaGetErrorString(e));
+    auto join = d128 ? by_type(cache->dtype, ppre::paged_join_kernel<__half, 128>, ppre::paged_join_kernel<__nv_bfloat16, 128>)
+                     : by_type(cache->dtype, ppre::paged_join_kernel<__half, 64>, ppre::paged_join_kernel<__nv_bfloat16, 64>);
+    e = launch_ex(join, dim3((unsigned)dev->sm_count, 2 * ppre::ROWS / ppre::JOIN_ROWS), dim3(ppre::JOIN_THREADS), 0, st, 1, p);
+    if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "attention join kernel launch: %s", cudaGetErrorString(e));
   }
   return W4A4_OK;
 }

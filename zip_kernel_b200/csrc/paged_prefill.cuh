@@ -40,7 +40,7 @@ static_assert(REG_ISSUE + 2 * REG_SOFTMAX <= 3 * 168, "the warpgroups share the 
 constexpr int TMEM_COLS = 512, TMEM_O = 256;
 constexpr float GROWTH = 8.f;                                // (log2) of a row's maximum before the output follows
 
-enum : int { SITE_PPRE_EMPTY = 80, SITE_PPRE_Q, SITE_PPRE_K, SITE_PPRE_V, SITE_PPRE_P, SITE_PPRE_S, SITE_PPRE_VZERO, SITE_PPRE_O, SITE_PPRE_QEMPTY, SITE_PPRE_OEMPTY, SITE_PPRE_WORK, SITE_PPRE_WFREE, SITE_PPRE_MEET };
+enum : int { SITE_PPRE_EMPTY = 80, SITE_PPRE_Q, SITE_PPRE_K, SITE_PPRE_V, SITE_PPRE_P, SITE_PPRE_S, SITE_PPRE_VZERO, SITE_PPRE_O, SITE_PPRE_QEMPTY, SITE_PPRE_OEMPTY, SITE_PPRE_WORK, SITE_PPRE_WFREE };
 
 template <int DIM>
 struct Layout {
@@ -50,7 +50,7 @@ struct Layout {
   static constexpr int q = STAGES * SLOT;
   static constexpr int works = q + 2 * SLOT;                 // Work [WORKS]
   static constexpr int bars = works + WORKS * 64;
-  static constexpr int total = bars + (2 * STAGES + 15 + 2 * WORKS) * 8 + 16;
+  static constexpr int total = bars + (2 * STAGES + 14 + 2 * WORKS) * 8 + 16;
   static constexpr int PART = 2 * ROWS * (DIM + 2);          // of a unit in the workspace: float2 m, l [row], float4 [dim / 4][row]
   static_assert(1024 + total <= 232448, "shared memory of one SM");
 };
@@ -63,14 +63,16 @@ struct Params {
   long long o_tok, o_head;
   float* lse;                 // (T, n_heads), or NULL
   float* parts;               // [2 * grid][Layout::PART]
-  int* arrived;               // [grid]: finished parts of the unit that is cut first in that run; zero between calls
+  void* joins;                // Join [grid]
   int n_heads, group, box, toks, min_rows;
   float scale_log2;
 };
 
 // A unit is a pair of row tiles of one (sequence, key/value head).  All units lie end to end, measured in slots: those that
 // a unit's last row sees and PAD more for what a unit costs besides its tiles; the row is cut into one equal run per
-// CTA.  A unit that falls into several runs is joined by the CTA that finishes its last part, in the order of the parts.
+// CTA.  A unit that falls into several runs leaves its parts in the workspace, and a second launch joins them in their
+// order, spread over the card.  (Joined by the CTA that finished a unit's last part, 64 tokens of 32/8 heads over 8192
+// slots took 48 us, half of it one CTA's reads of sixteen parts of 133 KB.)
 constexpr int PAD = 320;
 constexpr int MIN_RUN = 4 * TILE;                            // shorter runs cost more in joining than they save
 
@@ -183,10 +185,18 @@ struct Work {
   int q0, q_len, len;
   int j0, n_row[2];
   int whole;                  // the unit is in this run alone
-  int part, first_run, parts; // its part in the workspace; the run of its first part, and how many there are
-  int pad[2];
+  int part;                   // else its part in the workspace
+  int pad[4];
 };
 static_assert(sizeof(Work) == 64, "the place of one");
+
+// What the second launch needs to know of the unit that is cut for the first time at a run's end (there is one at most).
+struct Join {
+  int parts;                  // 0: none
+  int head, q0, q_len, tok0;
+  int pad[3];
+};
+static_assert(sizeof(Join) == 32, "the place of one");
 
 // descriptor of a B operand whose rows in shared memory are the K side (slots) and run along N (elements): 64 elements
 // under the 128-byte swizzle, 8 slots 1024 bytes apart, the next 64 elements `halves` bytes on
@@ -292,9 +302,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   uint64_t* o_empty = o_full + 2;
   uint64_t* w_full = o_empty + 2;                                // [WORKS]
   uint64_t* w_empty = w_full + WORKS;
-  uint64_t* meet = w_empty + WORKS;                              // the eight softmax warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet + 1);
-  int* last_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(w_empty + WORKS);
   grid_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -309,7 +317,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       mbar_init(&o_empty[i], 4);
     }
     for (int i = 0; i < WORKS; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 10); }
-    mbar_init(meet, 8);
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -354,6 +361,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         __syncwarp();
         ++nw;
       };
+      Join join{};
       if (run < runs) {
         const long long begin = run * all.total / runs, end = (run + 1) * all.total / runs;
         Unit u = unit_at(p, begin);
@@ -378,15 +386,21 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
           for (int t = 0; t < 2; ++t) w.n_row[t] = max(w.j0, min(j1, w.n_row[t]));
           w.whole = w.j0 == 0 && j1 == n;
-          // runs the unit falls into: run(x) = the c with c * total / runs <= x < (c + 1) * total / runs
-          w.first_run = (int)(((first + 1) * runs - 1) / all.total);
-          w.parts = (int)(((first + (long long)(n - 1) * TILE + 1) * runs - 1) / all.total) - w.first_run + 1;
           w.part = (int)(2 * run) + (first < begin ? 0 : 1);
+          if (w.j0 == 0 && j1 > 0 && j1 < n) {
+            // parts: the runs that the unit's tiles fall into; run(x) = the c with c * total / runs <= x < (c + 1) * total / runs
+            join.parts = (int)(((first + (long long)(n - 1) * TILE + 1) * runs - 1) / all.total - run) + 1;
+            join.head = u.head;
+            join.q0 = u.q.q0;
+            join.q_len = u.q.q_len;
+            join.tok0 = w.tok0;
+          }
           if (j1 > w.j0) put(w);
           if (u.u0 + u.weight >= end) break;
           next_unit(p, u);
         }
       }
+      if (lane == 0) static_cast<Join*>(p.joins)[run] = join;
       if (ok) put(Work{});
     } else if (warp == WARP_COPY) {
       // ---------------------------------------------------------- copies
@@ -516,14 +530,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem_base + lanes + t * TILE, to = tmem_base + lanes + TMEM_O + t * DIM;
-    uint32_t steps = 0, uses = 0, ring = 0, meetings = 0;  // ring: key and value tiles before this unit's
-    // (not a hardware barrier: a warp that gave up does not come again, and the others must not wait for ever)
-    auto all_meet = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(meet);
-      if (ok) ok = __all_sync(0xffffffffu, wide::wait_suspend(meet, meetings & 1, SITE_PPRE_MEET));
-      ++meetings;
-    };
+    uint32_t steps = 0, uses = 0, ring = 0;                // ring: key and value tiles before this unit's
     while (const Work* w = next_work()) {
       const int j0 = w->j0, n = w->n_row[t], len = w->len;
       float m = neg_inf(), l = 0.f;
@@ -619,9 +626,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           reinterpret_cast<uint4*>(dst_row + c)[i / 8] = make_uint4(pack2<T>(o[i] * f, o[i + 1] * f), pack2<T>(o[i + 2] * f, o[i + 3] * f),
                                                                     pack2<T>(o[i + 4] * f, o[i + 5] * f), pack2<T>(o[i + 6] * f, o[i + 7] * f));
       };
-      auto write_lse = [&]() {
-        if (p.lse) p.lse[tr * p.n_heads + hd] = l > 0.f ? (m + log2f(l)) * LN2 : l == l ? neg_inf() : l;
-      };
       const int pr = t * ROWS + row;                       // row of a part
       float* part = p.parts + (long long)w->part * L::PART;
       const bool whole = w->whole;
@@ -648,55 +652,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if (lane == 0) mbar_arrive(&o_empty[t]);
       }
       if (whole) {
-        if (live && ok) write_lse();
+        if (live && ok && p.lse) p.lse[tr * p.n_heads + hd] = l > 0.f ? (m + log2f(l)) * LN2 : l == l ? neg_inf() : l;
       } else {
         reinterpret_cast<float2*>(part)[pr] = make_float2(m, l);
-        const int parts = w->parts;
-        const long long c0 = w->first_run;
-        __threadfence();
-        all_meet();
-        if (tid == 0) {
-          int* a = p.arrived + c0;                         // (at most one unit is cut for the first time in a run)
-          const bool is_last = atomicAdd(a, 1) == parts - 1;
-          if (is_last) *a = 0;
-          __threadfence();
-          *last_flag = is_last;
-        }
-        all_meet();
-        if (ok && *last_flag && live) {
-          // the first part is the second of its run's two (the unit begins in that run), the others their run's first
-          auto part_of = [&](int k) { return p.parts + (2 * (c0 + k) + (k == 0 ? 1 : 0)) * L::PART; };
-          auto ml_of = [&](int k) { return __ldcg(reinterpret_cast<const float2*>(part_of(k)) + pr); };
-          m = neg_inf();
-          for (int k = 0; k < parts; ++k) m = fmaxf(m, ml_of(k).x);
-          l = 0.f;
-          float acc[DIM];
-#pragma unroll
-          for (int c = 0; c < DIM; ++c) acc[c] = 0.f;
-          for (int k = 0; k < parts; ++k) {
-            const float2 v = ml_of(k);
-            const float a = v.x == neg_inf() ? (v.y == v.y ? 0.f : 1.f) : ex2(v.x - m);
-            l += a * v.y;
-            const float4* src = reinterpret_cast<const float4*>(part_of(k) + 4 * ROWS) + pr;
-#pragma unroll
-            for (int c = 0; c < DIM; c += 4) {
-              const float4 o = __ldcg(src + c / 4 * (2 * ROWS));
-              acc[c] += a * o.x;
-              acc[c + 1] += a * o.y;
-              acc[c + 2] += a * o.z;
-              acc[c + 3] += a * o.w;
-            }
-          }
-          const float g = l > 0.f ? 1.f / l : 1.f;
-#pragma unroll
-          for (int c = 0; c < DIM; c += 16) {
-            float o[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = acc[c + i];
-            write_row(c, o, g);
-          }
-          write_lse();
-        }
       }
       work_done();
     }
@@ -713,6 +671,53 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     pre::tc_fence_after();
     pre::tmem_dealloc(tmem_base, TMEM_COLS);
   }
+}
+
+// Joins the parts of the units that the runs cut: a block takes JOIN_ROWS rows of the unit that is cut first in its run, a
+// thread EACH times four neighbouring elements.
+constexpr int JOIN_ROWS = 32, JOIN_THREADS = 256;
+template <typename T, int DIM>
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const Params p) {
+  using L = Layout<DIM>;
+  constexpr int STEP = JOIN_THREADS / JOIN_ROWS * 4;       // elements between a thread's fours
+  constexpr int EACH = DIM / STEP;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int run = blockIdx.x;
+  const Join u = static_cast<const Join*>(p.joins)[run];
+  const int row = blockIdx.y * JOIN_ROWS + threadIdx.x % JOIN_ROWS, c = threadIdx.x / JOIN_ROWS * 4;
+  const int t = row / ROWS, r = row % ROWS, tok = u.tok0 + t * p.toks + r / p.group;
+  if (u.parts == 0 || r / p.group >= p.toks || tok >= u.q_len) return;
+  // the first part is the second of its run's two (the unit begins in that run), the others their run's first
+  auto part_of = [&](int k) { return p.parts + (2 * (long long)(run + k) + (k == 0 ? 1 : 0)) * L::PART; };
+  float m = neg_inf(), l = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < u.parts; ++k) m = fmaxf(m, reinterpret_cast<const float2*>(part_of(k))[row].x);
+  float4 acc[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int k = 0; k < u.parts; ++k) {
+    const float2 ml = reinterpret_cast<const float2*>(part_of(k))[row];
+    const float a = ml.x == neg_inf() ? (ml.y == ml.y ? 0.f : 1.f) : ex2(ml.x - m);
+    l += a * ml.y;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const float4 o = reinterpret_cast<const float4*>(part_of(k) + 4 * ROWS)[(c + i * STEP) / 4 * (2 * ROWS) + row];
+      acc[i].x += a * o.x;
+      acc[i].y += a * o.y;
+      acc[i].z += a * o.z;
+      acc[i].w += a * o.w;
+    }
+  }
+  const float f = l > 0.f ? 1.f / l : 1.f;                 // (nothing summed: the sums are zero; a NaN stays one)
+  const long long tr = u.q0 + tok;
+  const int hd = u.head * p.group + r % p.group;
+  T* dst = static_cast<T*>(p.out) + tr * p.o_tok + (long long)hd * p.o_head + c;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    *reinterpret_cast<uint2*>(dst + i * STEP) = make_uint2(pack2<T>(acc[i].x * f, acc[i].y * f), pack2<T>(acc[i].z * f, acc[i].w * f));
+  if (p.lse && c == 0) p.lse[tr * p.n_heads + hd] = l > 0.f ? (m + log2f(l)) * LN2 : l == l ? neg_inf() : l;
 }
 
 }  // namespace ppre
