@@ -124,8 +124,11 @@ struct AttnPlan {
   int toks;                   // tokens of a row tile of the latter
   size_t few_parts, many_parts, joins, total;
 };
-// A sequence with up to this many rows (new tokens x heads of a group) goes to the kernel for few rows: one row tile of it.
-constexpr int ATTN_FEW_ROWS = pdec::ROWS;
+// A sequence with up to this many rows (new tokens x heads of a group) goes to the kernel for few rows: two row tiles of it,
+// the second of which finds keys and values in L2.  Measured, few against many rows: 32 sequences up to 4096 slots, 20
+// rows 59 to 90 us, 32 rows 83 to 103; 8 up to 32768, 32 rows 125 to 139; one of 8191, 32 rows 27 to 33; but 64 rows
+// 145 to 114, 236 to 168 and 37 to 33.
+constexpr int ATTN_FEW_ROWS = 2 * pdec::ROWS;
 
 AttnPlan attn_plan(const w4a4_paged_kv* c, int T, int n_heads, int max_q, int sm_count) {
   AttnPlan a{};

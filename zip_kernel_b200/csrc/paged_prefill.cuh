@@ -30,7 +30,6 @@ using namespace kv;
 using csum::add_f32x2;
 using csum::idesc_f16;
 using csum::umma_f16;
-using csum::wait_spin;
 
 constexpr int TILE = 128, ROWS = 128;                        // slots of a tile, rows of a row tile
 constexpr int WARP_COPY = 8, WARP_MMA = 9, WARP_PLAN = 10, THREADS = 12 * 32;
@@ -73,8 +72,11 @@ struct Params {
 // CTA.  A unit that falls into several runs leaves its parts in the workspace, and a second launch joins them in their
 // order, spread over the card.  (Joined by the CTA that finished a unit's last part, 64 tokens of 32/8 heads over 8192
 // slots took 48 us, half of it one CTA's reads of sixteen parts of 133 KB.)
+// (8192-token prompt: 528 us with 256, 523 with 320, 526 with 448)
 constexpr int PAD = 320;
-constexpr int MIN_RUN = 4 * TILE;                            // shorter runs cost more in joining than they save
+// Shorter runs cost more in joining than they save: 128 tokens of 32/8 heads over 1024 slots take 23.0 us with two tiles at
+// least, 26.3 with four and 32.8 with eight, 64 tokens over 8192 slots 34.6, 33.3 and 36.4.
+constexpr int MIN_RUN = 2 * TILE;
 
 struct Unit {
   int b, head, blk, blocks;
@@ -471,10 +473,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         mbar_arrive(&w_empty[nw++ % WORKS]);
         const int j_end = max(n_row[0], n_row[1]);
         if (j0 < j_end) {
-          ok = wait_spin(&full[s], ph, SITE_PPRE_K);
+          ok = wide::wait_suspend(&full[s], ph, SITE_PPRE_K);
           for (int t = 0; ok && t < 2; ++t) {
             if (n_row[t] == j0) continue;
-            ok = wait_spin(&q_full[t], uses[t] & 1, SITE_PPRE_Q);
+            ok = wide::wait_suspend(&q_full[t], uses[t] & 1, SITE_PPRE_Q);
             if (!ok) break;
             pre::tc_fence_after();
             scores(t, s, j0 + 1 == n_row[t]);
@@ -484,7 +486,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         }
         for (int j = j0; ok && j < j_end; ++j) {
           const int vs = s;
-          ok = wait_spin(&full[s], ph, SITE_PPRE_V);
+          ok = wide::wait_suspend(&full[s], ph, SITE_PPRE_V);
           next();
           const int ks = s;
           const uint32_t kph = ph;
@@ -498,7 +500,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             const uint64_t bd = smem_desc_mn_sw128(smem_u32(sm + vs * L::SLOT), TILE * 128);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (ok) ok = wait_spin(&p_full[2 * t + h], steps[t] & 1, SITE_PPRE_P);
+              if (ok) ok = wide::wait_suspend(&p_full[2 * t + h], steps[t] & 1, SITE_PPRE_P);
               if (!ok) break;
               pre::tc_fence_after();
 #pragma unroll
@@ -509,7 +511,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             ++steps[t];
             if (j == n_row[t] - 1) pre::umma_commit(&o_full[t]);
             if (j + 1 < n_row[t]) {
-              if (!k_here) ok = wait_spin(&full[ks], kph, SITE_PPRE_K);
+              if (!k_here) ok = wide::wait_suspend(&full[ks], kph, SITE_PPRE_K);
               k_here = true;
               if (!ok) break;
               pre::tc_fence_after();
