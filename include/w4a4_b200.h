@@ -374,7 +374,7 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
 
 /* Adds to sums[b, g, j] the attention weight that slot j of sequence b has received from the call's new tokens:
  * sum over the new tokens i that see j and the heads h of group g of exp(scale * q[i, h] . k[j] - lse[i, h]), lse from
- * w4a4_paged_attention.  sums: float, row strides in elements, max_pages * page_size (at least) floats a row; slots
+ * w4a4_paged_attention; at most 128 heads share a key/value head.  sums: float, row strides in elements, max_pages * page_size (at least) floats a row; slots
  * beyond a sequence's length are not touched. */
 int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
                            const int32_t* cu_seqlens, const int32_t* lengths, const float* lse, float* sums,

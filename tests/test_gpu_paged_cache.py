@@ -335,6 +335,29 @@ def test_long_history_of_one_sequence_and_many_short_ones():
     assert device_error() == 0
 
 
+@pytest.mark.parametrize("news,lens,heads,kv_heads,dim,page", [
+    ([2, 1, 40], [70, 33, 200], 130, 1, 64, 16),                          # more heads than a row tile of 128 has rows
+    ([40, 1, 0, 9] * 12, [90, 300, 7, 9] * 12, 4, 2, 64, 32),             # more sequences than a warp has lanes, both kernels
+    ([17] * 33, [17 + 5 * b for b in range(33)], 8, 4, 64, 16),
+    ([0, 0, 3], [5, 0, 3], 2, 2, 128, 16),
+])
+def test_attention_of_mixed_batches(news, lens, heads, kv_heads, dim, page):
+    from zip_kernel_b200 import ops
+    c = R.Case(news, lens, heads, kv_heads, dim, page, "fp16", seed=18)
+    ref, ref_lse, amp, mag = R.attention_ref(c)
+    q, kv, cu, n = c.q.to(DEV), c.kv(), c.cu.to(DEV), c.lengths.to(DEV)
+    out, lse = ops.paged_attention_cuda(q, kv, cu, n, return_lse=True)
+    R.assert_within(out, ref, R.attention_tolerance(c, ref, amp, mag), "out")
+    R.assert_within(lse, ref_lse, R.lse_tolerance(c, ref_lse, mag), "lse")
+    if heads // kv_heads <= 128:
+        want, rel = R.sums_ref(c, lse.cpu())
+        R.assert_within(ops.cache_weight_sums_cuda(q, kv, cu, n, lse), want, rel * want, "sums")
+    else:
+        with pytest.raises(RuntimeError, match="share"):
+            ops.cache_weight_sums_cuda(q, kv, cu, n, lse)
+    assert device_error() == 0
+
+
 def test_scores_that_grow_and_infinities():
     """Maxima that rise by more than 2^8 along a row (the output follows), rows of one weight, and a NaN key that only its
     own sequence's later rows see."""

@@ -11,8 +11,8 @@
 // more, and cut into one equal run per CTA; a tile goes through all row tiles before the next one, so its sums are
 // finished in one place.  Roles: a warp that issues copies, a thread that issues MMAs, two teams of four warps that read
 // the accumulators out, a team a tile.  Up to NARROW rows the queries' buffers are small and the keys' ring is deeper.
-// Measured with one team and four key tiles ahead: a decode step of 32 sequences up to 4096 slots 40 us, the last 64
-// tokens of four prompts up to 8000 slots 31 us.
+// Measured: a decode step of 32 sequences up to 4096 slots 33 us, the last 64 tokens of four prompts up to 8000 slots
+// 22.6 us; with one team and four key tiles ahead 40 and 31.
 #pragma once
 
 #include "paged_kv.cuh"
@@ -111,24 +111,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// Bounded wait that never sleeps, for the thread that issues the MMAs: it wakes from a sleeping wait about 450 clocks after
-// the arrival, and every hand-over between products and softmax would pay that.
-__device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity, int site) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (done) return true;
-    if ((i & 0xffff) == 0) {                               // (65536 polls are some milliseconds)
-      if (t0 == 0) t0 = wide::timer_ns();
-      else if (i > wide::WAIT_POLLS && wide::timer_ns() - t0 > wide::WAIT_NS) break;
-    }
-  }
-  record_error(site, parity);
-  return false;
-}
-
 template <typename T, int DIM, int COLS>
 __global__ void __launch_bounds__(THREADS, 1)
 cache_sums_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q, const Params p) {
@@ -218,7 +200,7 @@ cache_sums_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         while (ok) {
           const Part u(p, w, end);
           for (int t = u.first; ok && t < u.stop; ++t) {
-            ok = wait_spin(&k_full[ks], kph, SITE_SUMS_KFULL);
+            ok = wide::wait_suspend(&k_full[ks], kph, SITE_SUMS_KFULL);
             for (int r = 0; ok && r < u.n_rt; ++r) {
               const uint32_t step = team ? steps[1]++ : steps[0]++;
               const int acc = team * ACCS + (int)(step % ACCS);

@@ -7,18 +7,21 @@
 // products and softmax alternate: while the tensor cores work on one, the other's softmax warps have the CUDA cores.
 //
 // Roles: a warp that plans (finds the CTA's next unit of work and writes it to shared memory), a warp that issues copies
-// (TMA boxes of one page each), a thread that issues MMAs, four warps of softmax per row tile.  Scores are 128 x 128 fp32 in tensor memory, thread = row; the weights go back there as 16-bit pairs over
-// the scores and are the A operand of the second product, whose B operand is the value tile as it lands (slots x
-// elements, read along the elements).  The output stays in tensor memory; it is multiplied by exp(m_old - m_new) only
-// when some row's maximum has grown by more than a factor of 2^8, until when the weights are simply larger than one
-// (2^8 at most: exact in the sum, no worse rounded).  What a row's weights are rounded to (16 bits) is half a step of
-// the output's own type.
+// (TMA boxes of one page each), a thread that issues MMAs, four warps of softmax per row tile.  Scores are 128 x 128 fp32
+// in tensor memory, thread = row; the weights go back there as 16-bit pairs over the scores and are the A operand of the
+// second product, whose B operand is the value tile as it lands (slots x elements, read along the elements).  The output
+// stays in tensor memory; it is multiplied by exp(m_old - m_new) only when some row's maximum has grown by more than a
+// factor of 2^8, until when the weights are simply larger than one (2^8 at most: no worse rounded).  A weight is rounded
+// to the 16-bit type of the values, as the product demands: half a step of the output's own type.
 //
 // The order PV(j), S(j + 1) in the issuing thread makes one barrier do for two things: the scores of step j + 1 are
 // complete only after the product that reads the weights of step j and writes the output, so the softmax warps may
 // overwrite the one and multiply the other.
 //
-// What bounds it: products and exponentials alike, 2048 clocks each per step of both row tiles at dim 128.
+// What bounds it: products and exponentials alike at dim 128, 2048 clocks each per step of both row tiles if each had the SM to
+// itself.  A row tile's own chain - scores read 100, maximum 400, weights 1300 to 1500 beside the other tile's, then the
+// hand-over and its two products - makes a step 3400 to 3700 clocks; tensor memory is full (scores and outputs of both row
+// tiles), so the next scores cannot be made ahead.  Measured: 8192-token prompt, 32/8 heads, 524 us, 1050 TFLOP/s.
 #pragma once
 
 #include "cache_sums.cuh"
@@ -71,8 +74,9 @@ struct Params {
 // a unit's last row sees and PAD more for what a unit costs besides its tiles; the row is cut into one equal run per
 // CTA.  A unit that falls into several runs leaves its parts in the workspace, and a second launch joins them in their
 // order, spread over the card.  (Joined by the CTA that finished a unit's last part, 64 tokens of 32/8 heads over 8192
-// slots took 48 us, half of it one CTA's reads of sixteen parts of 133 KB.)
-// (8192-token prompt: 528 us with 256, 523 with 320, 526 with 448)
+// slots took 48 us, half of it one CTA's reads of sixteen parts of 133 KB.)  An 8192-token prompt takes 540, 525, 524 and 532 us
+// with a PAD of 192, 256, 320 and 448; chunks of 500, 333 and 166 tokens over up to 7001 slots
+// 119, 111, 107 and 109.
 constexpr int PAD = 320;
 // Shorter runs cost more in joining than they save: 128 tokens of 32/8 heads over 1024 slots take 23.0 us with two tiles at
 // least, 26.3 with four and 32.8 with eight, 64 tokens over 8192 slots 34.6, 33.3 and 36.4.

@@ -262,7 +262,7 @@ def cache_weight_sums_cuda(q: torch.Tensor, kv: PagedKV, cu_seqlens: torch.Tenso
                            scale: Optional[float] = None) -> torch.Tensor:
     """Adds the attention weight that each cache slot receives from the new tokens to ``sums (B, n_kv_heads, max_slots)``
     float32, in place, and returns it; ``None`` starts from zeros.  ``lse`` is what :func:`paged_attention_cuda` returned for the
-    same queries and lengths.  The heads that share a key/value head are added up.  Slots behind a sequence's length are
+    same queries and lengths.  The heads that share a key/value head, 128 at most, are added up.  Slots behind a sequence's length are
     left as they are.  To count the last tokens of a chunk only, pass their rows of ``q`` and ``lse`` and their
     ``cu_seqlens``."""
     q, T, n_heads, tok, head = _query_rows(kv, q)
