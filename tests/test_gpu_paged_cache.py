@@ -164,15 +164,15 @@ def test_captured_steps_replay_like_eager_ones_and_graphs_run_side_by_side():
             stream.synchronize()
             with torch.cuda.graph(graph, stream=stream):
                 decode_once(cache, qkv, cos, sin, out)
-        jobs.append((cache, out, hold, stream, graph, []))
+        jobs.append((cache, out, hold, stream, graph, [], qkv))        # (a graph keeps no tensor alive)
     torch.cuda.synchronize()
     for _ in range(4):
-        for cache, out, hold, stream, graph, outs in jobs:
+        for cache, out, hold, stream, graph, outs, _ in jobs:
             with torch.cuda.stream(stream):
                 graph.replay()
                 outs.append(out.clone())
     torch.cuda.synchronize()
-    for (cache, _, _, _, _, outs), (o, k, s) in zip(jobs, want):
+    for (cache, _, _, _, _, outs, _), (o, k, s) in zip(jobs, want):
         assert torch.equal(torch.stack(outs), o) and torch.equal(cache.k_pages, k) and torch.equal(cache.sums, s)
     assert device_error() == 0
 
@@ -415,3 +415,53 @@ def test_paged_stack_tracks_the_other_cache():
     assert ((y - x).float().norm() / x.float().norm()).item() < 0.3
     with pytest.raises(ValueError, match="paged"):
         ds.DecoderStack(small_cfg(qk_norm=True), 2, 32, DEV)
+
+
+def test_rotation_of_nothing_needs_no_tables_and_no_positions():
+    from zip_kernel_b200 import ops
+    c = R.Case([3, 1], [40, 7], 8, 2, 128, 16, "fp16", seed=19)
+    q, k, v, err = R.rope_ref(c, torch.zeros(64, 0), torch.zeros(64, 0))
+    for max_pos, interleaved in ((0, False), (0, True), (5, False)):
+        kv, none = c.kv(), torch.zeros(max_pos, 0, device=DEV)
+        got = ops.qkv_rope_cache_cuda(c.qkv.to(DEV), kv, c.cu.to(DEV), c.lengths.to(DEV), none, none, interleaved=interleaved)
+        R.assert_within(got, q, 0.0, "queries")
+        R.assert_within(kv.k_pages, k, 0.0, "keys")
+        R.assert_within(kv.v_pages, v, 0.0, "values")
+        assert device_error() == 0
+
+
+def test_sequences_without_any_page():
+    from zip_kernel_b200 import ops
+    c = R.Case([2, 1], [4, 7], 8, 2, 128, 16, "fp16", seed=20)
+    full, cu, n, q = c.kv(), c.cu.to(DEV), torch.zeros(2, dtype=torch.int32, device=DEV), c.q.to(DEV)
+    kv = ops.PagedKV(full.k_pages, full.v_pages, full.block_table[:, :0])
+    out, lse = ops.paged_attention_cuda(q, kv, cu, n, return_lse=True)
+    assert (out == 0).all() and (lse == float("-inf")).all()
+    assert ops.cache_weight_sums_cuda(q, kv, cu, n, lse).shape == (2, 2, 0)
+    assert device_error() == 0
+    with pytest.raises(ValueError, match="budget"):
+        ops.cache_evict_cuda(kv, n, torch.zeros(2, 2, 0, device=DEV), 1)
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [5, 2, 1], [700, 3, 150]])
+def test_attention_may_overwrite_its_queries(news):
+    from zip_kernel_b200 import ops
+    c = R.Case(news, [2000, 77, 900], 10, 2, 128, 16, "bf16", seed=21)
+    kv, cu, n = c.kv(), c.cu.to(DEV), c.lengths.to(DEV)
+    want, q = ops.paged_attention_cuda(c.q.to(DEV), kv, cu, n), c.q.to(DEV)
+    got = ops.paged_attention_cuda(q, kv, cu, n, out=q)
+    assert got is q and torch.equal(got, want)
+
+
+def test_offsets_of_a_captured_step_are_whole_before_its_replay():
+    from zip_kernel_b200.paged_cache import PagedKVCache
+    cache = PagedKVCache(1, 3, 64, 2, 64, page_size=16, device=DEV)
+    torch.empty(1 << 20, device=DEV).fill_(1e30)             # what fresh memory may hold
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        cache.cu_seqlens(5)
+    assert cache.cu_seqlens(5).tolist() == [0, 5, 10, 15] and cache.cu_seqlens(1).tolist() == [0, 1, 2, 3]
+    for bad in (0, 8, 24, -16):
+        with pytest.raises(ValueError, match="page_size"):
+            PagedKVCache(1, 3, 64, 2, 64, page_size=bad, device=DEV)

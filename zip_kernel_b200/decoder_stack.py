@@ -241,6 +241,8 @@ class DecoderStack:
 
 def run(cfg: StackConfig, batch: int, prefill_len: int, decode_steps: int, device, use_graph: bool = True, seed: int = 0,
         prepared: bool = True, fused_seams: bool = True, paged: bool = False, chunk: int = 0, evict: int = 0):
+    if chunk < 0 or evict < 0:
+        raise ValueError(f"chunk ({chunk}) and evict ({evict}) must not be negative")
     if (chunk or evict) and not paged:
         raise ValueError("chunk and evict need paged=True")
     max_len = prefill_len + decode_steps

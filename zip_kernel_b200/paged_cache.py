@@ -8,7 +8,7 @@ decode step can be captured in a CUDA graph and replayed.  No counterpart in the
 
 from __future__ import annotations
 
-from typing import Dict, Optional
+from typing import Optional
 
 import torch
 
@@ -26,6 +26,8 @@ class PagedKVCache:
                  dtype=torch.float16, device="cuda", track_weights: bool = False):
         if n_layers < 1 or n_seqs < 1 or max_slots < 1:
             raise ValueError(f"layers ({n_layers}), sequences ({n_seqs}) and slots ({max_slots}) must be positive")
+        if page_size < 16 or page_size % 16:
+            raise ValueError(f"page_size must be a positive multiple of 16, got {page_size}")
         cols = (max_slots + page_size - 1) // page_size
         n_pages = n_seqs * cols
         shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
@@ -43,17 +45,15 @@ class PagedKVCache:
         self.sums: Optional[torch.Tensor] = None
         if track_weights:
             self.sums = torch.zeros((n_layers, n_seqs, n_kv_heads, self.max_slots), dtype=torch.float32, device=self.device)
-        self._cu: Dict[int, torch.Tensor] = {}
+        self._ones = torch.arange(n_seqs + 1, dtype=torch.int32, device=self.device)
 
     def layer(self, i: int) -> ops.PagedKV:
         return self.layers[i]
 
     def cu_seqlens(self, q_len: int) -> torch.Tensor:
-        """Offsets of a step in which every sequence has ``q_len`` new tokens."""
-        cu = self._cu.get(q_len)
-        if cu is None:
-            cu = self._cu[q_len] = torch.arange(self.n_seqs + 1, dtype=torch.int32, device=self.device) * q_len
-        return cu
+        """Offsets of a step in which every sequence has ``q_len`` new tokens.  Made on the current stream at every call, but for
+        the one of single tokens: a tensor kept from a capture would be empty until the graph's first replay."""
+        return self._ones if q_len == 1 else self._ones * q_len
 
     def advance(self, q_len: int) -> torch.Tensor:
         """Makes room for ``q_len`` new tokens of every sequence (once per step, before its first layer) and returns the
