@@ -351,7 +351,7 @@ typedef struct w4a4_paged_kv {
  * rotation (a, b) -> (a c - b s, b c + a s) of the first rot_dim elements (a multiple of 16; pairs are neighbours when
  * interleaved, else i and i + rot_dim / 2), queries to q_out (T, n_heads, head_dim), keys and values to their cache
  * slots.  cos and sin (max_pos, rot_dim / 2) float; a token's position is its slot, plus offsets[b] where offsets is
- * given (slots that were evicted).  One rounding per value.  q_out may be the query columns of qkv. */
+ * given (slots that were evicted); with rot_dim 0 neither tables nor positions count.  One rounding per value.  q_out may be the query columns of qkv. */
 int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long ld_qkv, const int32_t* cu_seqlens,
                         const int32_t* lengths, const float* cos, const float* sin, int max_pos, int rot_dim,
                         const void* q_norm, const void* k_norm, float eps, int interleaved, const int32_t* offsets,

@@ -325,7 +325,7 @@ int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long 
   const long long slots = (long long)cache->max_pages * cache->page_size;
   CHECK_ARG((sums_head_stride >= slots || cache->n_kv_heads == 1) && (sums_seq_stride >= slots || cache->n_seqs <= 1),
             "sums strides (%lld, %lld) are below the %lld slots of a row", sums_seq_stride, sums_head_stride, slots);
-  if (T == 0 || cache->n_seqs == 0 || max_q_len == 0) return W4A4_OK;
+  if (T == 0 || cache->n_seqs == 0 || max_q_len == 0 || slots == 0) return W4A4_OK;
   rc = check_rows("q", q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
   if (rc) return rc;
   CHECK_ARG(lse && sums, "lse or sums is NULL");

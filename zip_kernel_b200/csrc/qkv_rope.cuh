@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopePar
   const Seq q = load_seq(p.s, b);
   const int slot = q.len - q.q_len + (t - q.q0);
   const int pos = slot + (p.offsets ? ld_plain(p.offsets + b) : 0);
-  if (slot < 0 || (unsigned)pos >= (unsigned)p.max_pos || t < q.q0 || t >= q.q0 + q.q_len) {
+  if (slot < 0 || (p.rot > 0 && (unsigned)pos >= (unsigned)p.max_pos) || t < q.q0 || t >= q.q0 + q.q_len) {
     if (lane == 0) record_error(SITE_KV_POS, b);
     return;
   }

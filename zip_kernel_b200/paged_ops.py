@@ -11,6 +11,7 @@ the end of the last, and ``lengths (B)``, the cache slots in use with the new to
 sequence ``b`` has slot ``lengths[b] - q_len[b] + i`` and sees the slots up to its own.  Their values stay on the device: what
 is out of range there is cut or left out and sets the device error word (``_lib.device_error``), see
 include/w4a4_b200.h.  Every call is issued on the current stream of the cache's device and can be captured in a graph.
+Forward only: no gradient is recorded.
 
 No counterpart in the reference, whose layer harness uses PyTorch here (bench/layer/qwen3_layer_bf16.py:129-241).
 """
@@ -170,7 +171,7 @@ def qkv_rope_cache_cuda(qkv: torch.Tensor, kv: PagedKV, cu_seqlens: torch.Tensor
     key heads (where ``q_norm`` / ``k_norm (head_dim)`` are given), rotation of their first ``2 * cos.shape[1]`` elements,
     keys and values written to their cache slots.  Returns the queries ``(T, n_heads, head_dim)``.
 
-    ``cos``, ``sin``: float32 ``(max_pos, rot_dim / 2)``.  A token's position is its cache slot, plus ``offsets[b]`` (int32) where
+    ``cos``, ``sin``: float32 ``(max_pos, rot_dim / 2)``; of width 0 nothing is rotated.  A token's position is its cache slot, plus ``offsets[b]`` (int32) where
     that is given: the number of slots evicted from the sequence.  ``interleaved``: pairs are neighbours, else ``i`` and
     ``i + rot_dim / 2``.  Everything is computed in float32 and rounded once.  Tokens behind the last sequence are left as
     ``out`` holds them (undefined without ``out``); ``out`` may be the query columns of ``qkv``."""
@@ -224,7 +225,7 @@ def paged_attention_cuda(q: torch.Tensor, kv: PagedKV, cu_seqlens: torch.Tensor,
 
     ``scale``: of the scores, ``head_dim ** -0.5`` by default.  ``max_q_len``: no sequence has more new tokens (``T`` by
     default); pass 1 for a decode step, so that only the kernel for few rows is launched.  A row that sees no slot is
-    zero, its ``lse`` minus infinity.  Tokens behind the last sequence are left as ``out`` holds them (undefined without
+    zero, its ``lse`` minus infinity.  ``out`` may be ``q``.  Tokens behind the last sequence are left as ``out`` holds them (undefined without
     ``out``, like their ``lse``).  Values within a sequence's length must be finite; what lies behind it does not matter."""
     q, T, n_heads, tok, head = _query_rows(kv, q)
     _check_seqs(kv, cu_seqlens, lengths)
