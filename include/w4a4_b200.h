@@ -374,12 +374,17 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
 
 /* Adds to sums[b, g, j] the attention weight that slot j of sequence b has received from the call's new tokens:
  * sum over the new tokens i that see j and the heads h of group g of exp(scale * q[i, h] . k[j] - lse[i, h]), lse from
- * w4a4_paged_attention; at most 128 heads share a key/value head.  sums: float, row strides in elements, max_pages * page_size (at least) floats a row; slots
- * beyond a sequence's length are not touched. */
+ * w4a4_paged_attention; at most 128 heads share a key/value head.  sums: float, row strides in elements, at least
+ * max_pages * page_size floats a row; slots beyond a sequence's length are not touched.  _fresh: sums holds nothing yet;
+ * the same as on zeros, every slot of every row is written (T and max_q_len must be positive then). */
 int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
                            const int32_t* cu_seqlens, const int32_t* lengths, const float* lse, float* sums,
                            long long sums_seq_stride, long long sums_head_stride, int T, int n_heads, int max_q_len,
                            float scale, void* stream);
+int w4a4_cache_weight_sums_fresh(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
+                                 const int32_t* cu_seqlens, const int32_t* lengths, const float* lse, float* sums,
+                                 long long sums_seq_stride, long long sums_head_stride, int T, int n_heads, int max_q_len,
+                                 float scale, void* stream);
 
 /* Keeps, for every sequence and key/value head on its own, n_sink first slots, n_recent last ones and those with the
  * largest sums in between, `budget` in all (equal sums: the lowest slots first; NaN counts as the least), and moves

@@ -465,3 +465,21 @@ def test_offsets_of_a_captured_step_are_whole_before_its_replay():
     for bad in (0, 8, 24, -16):
         with pytest.raises(ValueError, match="page_size"):
             PagedKVCache(1, 3, 64, 2, 64, page_size=bad, device=DEV)
+
+
+@pytest.mark.parametrize("news,lens,max_pages,tail", [
+    ([1, 1, 0, 1], [70, 1, 40, 0], 300, 0),                  # chunks of zeros behind the lengths, a sequence without a new token
+    ([0, 40, 3], [128, 300, 9], None, 2), ([0, 0], [20, 0], 2, 3), ([1] * 40, [1 + 7 * b for b in range(40)], 20, 0),
+    ([5, 2], [3, 1], 2, 0),
+])
+def test_sums_that_hold_nothing_yet_are_written_whole(news, lens, max_pages, tail):
+    from zip_kernel_b200 import ops
+    c = R.Case(news, lens, 8, 2, 128, 16, "fp16", seed=22, max_pages=max_pages, tail=tail)
+    q, kv, cu, n = c.q.to(DEV), c.kv(), c.cu.to(DEV), c.lengths.to(DEV)
+    lse = ops.paged_attention_cuda(q, kv, cu, n, return_lse=True)[1]
+    want = ops.cache_weight_sums_cuda(q, kv, cu, n, lse, torch.zeros(c.n, 2, kv.max_slots, device=DEV))
+    hold = torch.full((c.n, 2, kv.max_slots), float("nan"), device=DEV)
+    del hold                                                 # the memory that the next sums most likely get
+    got = ops.cache_weight_sums_cuda(q, kv, cu, n, lse)
+    assert torch.equal(got, want) and device_error() == 0
+    assert torch.equal(ops.cache_weight_sums_cuda(q[:0], kv, torch.zeros_like(cu), n, lse[:0]), torch.zeros_like(want))

@@ -110,3 +110,13 @@ def test_cache_handle_refuses_host_tensors():
     pages = torch.zeros(4, 2, 16, 128, dtype=torch.float16)
     with pytest.raises(ValueError, match="CUDA"):
         ops.PagedKV(pages, pages, torch.zeros(1, 2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("kw,word", [(dict(T=0), "no new token"), (dict(max_q=0), "no new token"), (dict(T=-1), "negative"), (dict(n_heads=12), "multiple")])
+def test_sums_that_hold_nothing_need_a_new_token(kw, word):
+    from zip_kernel_b200 import _lib
+    L, d = _lib.load(), dict(T=3, n_heads=32, max_q=1)
+    d.update(kw)
+    kv = arg()
+    assert L.w4a4_cache_weight_sums_fresh(ctypes.addressof(kv), P, 4096, 128, P, P, P, P, 8 * 64, 64, d["T"], d["n_heads"], d["max_q"], 0.1, None) == BAD
+    assert word in L.w4a4_last_error().decode()

@@ -64,6 +64,7 @@ SIGNATURES = {
     "w4a4_paged_attention_workspace_bytes": (_SZ, [_PTR, _INT, _INT, _INT]),
     "w4a4_paged_attention": (_INT, [_PTR, _PTR, _LL, _LL, _PTR, _PTR, _PTR, _LL, _LL, _PTR, _INT, _INT, _INT, _c.c_float, _PTR, _SZ, _PTR]),
     "w4a4_cache_weight_sums": (_INT, [_PTR, _PTR, _LL, _LL] + [_PTR] * 4 + [_LL, _LL, _INT, _INT, _INT, _c.c_float, _PTR]),
+    "w4a4_cache_weight_sums_fresh": (_INT, [_PTR, _PTR, _LL, _LL] + [_PTR] * 4 + [_LL, _LL, _INT, _INT, _INT, _c.c_float, _PTR]),
     "w4a4_cache_evict": (_INT, [_PTR] * 4 + [_LL, _LL, _INT, _INT, _INT] + [_PTR] * 4),
 }
 

@@ -11,8 +11,8 @@
 // more, and cut into one equal run per CTA; a tile goes through all row tiles before the next one, so its sums are
 // finished in one place.  Roles: a warp that issues copies, a thread that issues MMAs, two teams of four warps that read
 // the accumulators out, a team a tile.  Up to NARROW rows the queries' buffers are small and the keys' ring is deeper.
-// Measured: a decode step of 32 sequences up to 4096 slots 33 us, the last 64 tokens of four prompts up to 8000 slots
-// 22.6 us; with one team and four key tiles ahead 40 and 31.
+// Measured: a decode step of 32 sequences up to 4096 slots 31 us, the last 64 tokens of four prompts up to 8000 slots
+// 20.6 us, sums fresh; zeroed by a launch of their own, with one team and four key tiles ahead, 40 and 31.
 #pragma once
 
 #include "paged_kv.cuh"
@@ -54,6 +54,7 @@ struct Params {
   long long sums_seq, sums_head;
   int n_heads, group, box;
   int cols, toks;             // rows of a row tile on the N side, and whole tokens in it
+  int fresh;                  // sums holds nothing yet: every slot is written, zero where nothing is added
   float scale_log2;
 };
 
@@ -75,6 +76,22 @@ struct Part {
     more = w.at - w.tile + stop_step < end;
   }
 };
+
+// Zeros behind the lengths, and in all of a sequence without a new token, of sums that hold nothing yet.  The read-out
+// warps write them while the first keys are on their way.  Measured, a decode step of 32 sequences up to 4096 slots of 8
+// heads, 31 us; 33 with a launch before that zeroes all of sums.
+__device__ __forceinline__ void zero_rest(const Params& p) {
+  constexpr int CHUNK = 4096;
+  const int n_chunks = (p.s.max_slots + CHUNK - 1) / CHUNK;
+  const long long all = (long long)p.s.n * p.c.n_kv * n_chunks;
+  for (long long i = blockIdx.x; i < all; i += gridDim.x) {
+    const int row = (int)(i / n_chunks), c0 = (int)(i - (long long)row * n_chunks) * CHUNK, b = row / p.c.n_kv;
+    const Seq q = load_seq(p.s, b);
+    float* s = p.sums + (long long)b * p.sums_seq + (long long)(row % p.c.n_kv) * p.sums_head;
+    const int end = c0 + min(CHUNK, p.s.max_slots - c0);
+    for (int j = max(c0, q.q_len > 0 ? q.len : 0) + threadIdx.x; j < end; j += WARPS * 32) s[j] = 0.f;
+  }
+}
 
 // kind::f16: 16-bit operands K-major in shared memory, M = 128, fp32 accumulation
 template <typename T>
@@ -147,6 +164,7 @@ cache_sums_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   else grid_dependency_wait();
 
   bool ok = true;                                          // no wait of this thread has given up
+  if (p.fresh && warp < WARPS) zero_rest(p);
   Walk<Params> w;
   long long total, runs, begin, end;
   if (w.start(p, gridDim.x, blockIdx.x, total, runs, begin, end)) {
@@ -312,7 +330,8 @@ cache_sums_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           }
           if (ok && slot < w.q.len) {
             const float2 s = unpack_f32x2(add_f32x2(sum2[0], sum2[1]));
-            p.sums[(long long)w.b * p.sums_seq + (long long)w.head * p.sums_head + slot] += sum + (s.x + s.y);
+            float* to = p.sums + (long long)w.b * p.sums_seq + (long long)w.head * p.sums_head + slot;
+            *to = (p.fresh ? 0.f : *to) + (sum + (s.x + s.y));
           }
         }
         if (!u.more) break;

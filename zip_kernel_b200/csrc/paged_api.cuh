@@ -148,6 +148,66 @@ AttnPlan attn_plan(const w4a4_paged_kv* c, int T, int n_heads, int max_q, int sm
   return a;
 }
 
+int weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
+                const int32_t* cu_seqlens, const int32_t* lengths, const float* lse, float* sums, long long sums_seq_stride,
+                long long sums_head_stride, int T, int n_heads, int max_q_len, float scale, bool fresh, void* stream) {
+  begin_call();
+  int rc = check_cache(cache);
+  if (!rc) rc = check_seqs(cache, cu_seqlens, lengths, T, n_heads);
+  if (rc) return rc;
+  CHECK_ARG(max_q_len >= 0, "max_q_len must not be negative, got %d", max_q_len);
+  CHECK_ARG(scale > 0.f && scale < 3e38f, "scale must be positive and finite, got %g", (double)scale);
+  const int group = n_heads / cache->n_kv_heads;
+  if (group > csum::MAX_COLS) return fail(W4A4_ERR_UNSUPPORTED, "%d heads share a key/value head; at most %d", group, csum::MAX_COLS);
+  const long long slots = (long long)cache->max_pages * cache->page_size;
+  CHECK_ARG((sums_head_stride >= slots || cache->n_kv_heads == 1) && (sums_seq_stride >= slots || cache->n_seqs <= 1),
+            "sums strides (%lld, %lld) are below the %lld slots of a row", sums_seq_stride, sums_head_stride, slots);
+  if (T == 0 || cache->n_seqs == 0 || max_q_len == 0 || slots == 0) return W4A4_OK;
+  rc = check_rows("q", q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
+  if (rc) return rc;
+  CHECK_ARG(lse && sums, "lse or sums is NULL");
+  if (!aligned(lse, 4) || !aligned(sums, 4)) return fail(W4A4_ERR_ALIGNMENT, "lse and sums must be 4-byte aligned");
+  DeviceInfo* dev = nullptr;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  max_q_len = max_q_len < T ? max_q_len : T;
+  csum::Params p;
+  p.c = device_cache(cache);
+  p.s = device_seqs(cache, cu_seqlens, lengths, T, max_q_len);
+  p.lse = lse;
+  p.sums = sums;
+  p.sums_seq = sums_seq_stride;
+  p.sums_head = sums_head_stride;
+  p.n_heads = n_heads;
+  p.group = group;
+  p.box = box_slots(cache->page_size, csum::TILE);
+  // the narrowest product that takes all rows of the longest sequence, 128 at most
+  const long long rows = (long long)max_q_len * group;
+  p.cols = rows >= csum::MAX_COLS ? csum::MAX_COLS : (int)((rows + 15) / 16 * 16);
+  p.toks = p.cols / group;
+  p.scale_log2 = scale * kv::LOG2E;
+  p.fresh = fresh;
+  CUtensorMap tk, tq;
+  rc = make_cache_map(&tk, cache, false, p.box);
+  if (!rc) rc = make_query_map(&tq, q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim, cache->dtype, group, p.toks);
+  if (rc) return rc;
+  const bool d128 = cache->head_dim == 128;
+  auto launch = [&](auto k64h, auto k64b, auto k128h, auto k128b, size_t smem) {
+    auto kern = d128 ? by_type(cache->dtype, k128h, k128b) : by_type(cache->dtype, k64h, k64b);
+    return launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(csum::THREADS), smem, static_cast<cudaStream_t>(stream), 1, tk, tq, p);
+  };
+  constexpr int N = csum::NARROW, M = csum::MAX_COLS;
+  const cudaError_t e =
+      p.cols <= N ? launch(csum::cache_sums_kernel<__half, 64, N>, csum::cache_sums_kernel<__nv_bfloat16, 64, N>,
+                           csum::cache_sums_kernel<__half, 128, N>, csum::cache_sums_kernel<__nv_bfloat16, 128, N>,
+                           d128 ? csum::smem_bytes<128, N>() : csum::smem_bytes<64, N>())
+                  : launch(csum::cache_sums_kernel<__half, 64, M>, csum::cache_sums_kernel<__nv_bfloat16, 64, M>,
+                           csum::cache_sums_kernel<__half, 128, M>, csum::cache_sums_kernel<__nv_bfloat16, 128, M>,
+                           d128 ? csum::smem_bytes<128, M>() : csum::smem_bytes<64, M>());
+  if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "weight sums kernel launch: %s", cudaGetErrorString(e));
+  return W4A4_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -314,60 +374,20 @@ int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long 
                            const int32_t* cu_seqlens, const int32_t* lengths, const float* lse, float* sums,
                            long long sums_seq_stride, long long sums_head_stride, int T, int n_heads, int max_q_len,
                            float scale, void* stream) {
-  begin_call();
-  int rc = check_cache(cache);
-  if (!rc) rc = check_seqs(cache, cu_seqlens, lengths, T, n_heads);
-  if (rc) return rc;
-  CHECK_ARG(max_q_len >= 0, "max_q_len must not be negative, got %d", max_q_len);
-  CHECK_ARG(scale > 0.f && scale < 3e38f, "scale must be positive and finite, got %g", (double)scale);
-  const int group = n_heads / cache->n_kv_heads;
-  if (group > csum::MAX_COLS) return fail(W4A4_ERR_UNSUPPORTED, "%d heads share a key/value head; at most %d", group, csum::MAX_COLS);
-  const long long slots = (long long)cache->max_pages * cache->page_size;
-  CHECK_ARG((sums_head_stride >= slots || cache->n_kv_heads == 1) && (sums_seq_stride >= slots || cache->n_seqs <= 1),
-            "sums strides (%lld, %lld) are below the %lld slots of a row", sums_seq_stride, sums_head_stride, slots);
-  if (T == 0 || cache->n_seqs == 0 || max_q_len == 0 || slots == 0) return W4A4_OK;
-  rc = check_rows("q", q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
-  if (rc) return rc;
-  CHECK_ARG(lse && sums, "lse or sums is NULL");
-  if (!aligned(lse, 4) || !aligned(sums, 4)) return fail(W4A4_ERR_ALIGNMENT, "lse and sums must be 4-byte aligned");
-  DeviceInfo* dev = nullptr;
-  rc = current_device(&dev);
-  if (rc) return rc;
-  max_q_len = max_q_len < T ? max_q_len : T;
-  csum::Params p;
-  p.c = device_cache(cache);
-  p.s = device_seqs(cache, cu_seqlens, lengths, T, max_q_len);
-  p.lse = lse;
-  p.sums = sums;
-  p.sums_seq = sums_seq_stride;
-  p.sums_head = sums_head_stride;
-  p.n_heads = n_heads;
-  p.group = group;
-  p.box = box_slots(cache->page_size, csum::TILE);
-  // the narrowest product that takes all rows of the longest sequence, 128 at most
-  const long long rows = (long long)max_q_len * group;
-  p.cols = rows >= csum::MAX_COLS ? csum::MAX_COLS : (int)((rows + 15) / 16 * 16);
-  p.toks = p.cols / group;
-  p.scale_log2 = scale * kv::LOG2E;
-  CUtensorMap tk, tq;
-  rc = make_cache_map(&tk, cache, false, p.box);
-  if (!rc) rc = make_query_map(&tq, q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim, cache->dtype, group, p.toks);
-  if (rc) return rc;
-  const bool d128 = cache->head_dim == 128;
-  auto launch = [&](auto k64h, auto k64b, auto k128h, auto k128b, size_t smem) {
-    auto kern = d128 ? by_type(cache->dtype, k128h, k128b) : by_type(cache->dtype, k64h, k64b);
-    return launch_ex(kern, dim3((unsigned)dev->sm_count), dim3(csum::THREADS), smem, static_cast<cudaStream_t>(stream), 1, tk, tq, p);
-  };
-  constexpr int N = csum::NARROW, M = csum::MAX_COLS;
-  const cudaError_t e =
-      p.cols <= N ? launch(csum::cache_sums_kernel<__half, 64, N>, csum::cache_sums_kernel<__nv_bfloat16, 64, N>,
-                           csum::cache_sums_kernel<__half, 128, N>, csum::cache_sums_kernel<__nv_bfloat16, 128, N>,
-                           d128 ? csum::smem_bytes<128, N>() : csum::smem_bytes<64, N>())
-                  : launch(csum::cache_sums_kernel<__half, 64, M>, csum::cache_sums_kernel<__nv_bfloat16, 64, M>,
-                           csum::cache_sums_kernel<__half, 128, M>, csum::cache_sums_kernel<__nv_bfloat16, 128, M>,
-                           d128 ? csum::smem_bytes<128, M>() : csum::smem_bytes<64, M>());
-  if (e != cudaSuccess) return fail(W4A4_ERR_LAUNCH, "weight sums kernel launch: %s", cudaGetErrorString(e));
-  return W4A4_OK;
+  return weight_sums(cache, q, q_tok_stride, q_head_stride, cu_seqlens, lengths, lse, sums, sums_seq_stride, sums_head_stride, T,
+                     n_heads, max_q_len, scale, false, stream);
+}
+
+int w4a4_cache_weight_sums_fresh(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,
+                                 const int32_t* cu_seqlens, const int32_t* lengths, const float* lse, float* sums,
+                                 long long sums_seq_stride, long long sums_head_stride, int T, int n_heads, int max_q_len,
+                                 float scale, void* stream) {
+  if (T == 0 || max_q_len == 0) {
+    begin_call();
+    return fail(W4A4_ERR_BAD_ARG, "no new token: nothing would be written");
+  }
+  return weight_sums(cache, q, q_tok_stride, q_head_stride, cu_seqlens, lengths, lse, sums, sums_seq_stride, sums_head_stride, T,
+                     n_heads, max_q_len, scale, true, stream);
 }
 
 int w4a4_cache_evict(const w4a4_paged_kv* cache, const w4a4_paged_kv* into, const int32_t* lengths, const float* sums,

@@ -271,15 +271,18 @@ def cache_weight_sums_cuda(q: torch.Tensor, kv: PagedKV, cu_seqlens: torch.Tenso
     if lse.shape != (T, n_heads) or lse.dtype is not torch.float32 or lse.device != kv.device:
         raise ValueError(f"lse must be float32 ({T}, {n_heads}) on {kv.device}, got {lse.dtype} {tuple(lse.shape)} on {lse.device}")
     scale = _check_scale(kv, scale)
-    if sums is None:
-        sums = torch.zeros(kv._sums_shape, dtype=torch.float32, device=kv.device)
-    seq, group = _check_sums(kv, sums)
     max_q = _max_q(max_q_len, T)
-    if T and kv.n_seqs and max_q:
+    some, add = T and kv.n_seqs and max_q, _L.w4a4_cache_weight_sums
+    if sums is not None:
+        seq, group = _check_sums(kv, sums)
+    else:
+        sums = (torch.empty if some else torch.zeros)(kv._sums_shape, dtype=torch.float32, device=kv.device)
+        seq, group, add = kv.n_kv_heads * kv.max_slots, kv.max_slots, _L.w4a4_cache_weight_sums_fresh
+    if some:
         lse = lse.contiguous()
         device = kv.device
         with _lib.on_device(device):
-            status = _L.w4a4_cache_weight_sums(
+            status = add(
                 kv._ptr, q.data_ptr(), tok, head, cu_seqlens.data_ptr(), lengths.data_ptr(), lse.data_ptr(), sums.data_ptr(), seq, group,
                 T, n_heads, max_q, scale, _lib.stream_ptr(device))
         if status:
