@@ -19,9 +19,11 @@
 // overwrite the one and multiply the other.
 //
 // What bounds it: products and exponentials alike at dim 128, 2048 clocks each per step of both row tiles if each had the SM to
-// itself.  A row tile's own chain - scores read 100, maximum 400, weights 1300 to 1500 beside the other tile's, then the
-// hand-over and its two products - makes a step 3400 to 3700 clocks; tensor memory is full (scores and outputs of both row
-// tiles), so the next scores cannot be made ahead.  Measured: 8192-token prompt, 32/8 heads, 524 us, 1050 TFLOP/s.
+// itself.  A row tile's own chain is longer - scores read 100, maximum 400, weights 1300 to 1500 beside the other tile's,
+// then the hand-over and its products - and tensor memory is full (scores and outputs of both row tiles), so the next
+// scores cannot be made ahead: a step takes about 3200 clocks.  Measured: 8192-token prompt, 32/8 heads, 491 us, 1120
+// TFLOP/s.  One thread issues the products of both row tiles, in turn: with a thread for each the two fall into step and
+// no longer fill each other's pauses (607 us).
 #pragma once
 
 #include "cache_sums.cuh"
@@ -37,7 +39,7 @@ using csum::umma_f16;
 constexpr int TILE = 128, ROWS = 128;                        // slots of a tile, rows of a row tile
 constexpr int WARP_COPY = 8, WARP_MMA = 9, WARP_PLAN = 10, THREADS = 12 * 32;
 constexpr int WORKS = 4;                                     // units planned ahead
-constexpr int REG_ISSUE = 72, REG_SOFTMAX = 216;
+constexpr int REG_ISSUE = 88, REG_SOFTMAX = 208;
 static_assert(REG_ISSUE + 2 * REG_SOFTMAX <= 3 * 168, "the warpgroups share the registers of the launch");
 constexpr int TMEM_COLS = 512, TMEM_O = 256;
 constexpr float GROWTH = 8.f;                                // (log2) of a row's maximum before the output follows
@@ -74,9 +76,8 @@ struct Params {
 // a unit's last row sees and PAD more for what a unit costs besides its tiles; the row is cut into one equal run per
 // CTA.  A unit that falls into several runs leaves its parts in the workspace, and a second launch joins them in their
 // order, spread over the card.  (Joined by the CTA that finished a unit's last part, 64 tokens of 32/8 heads over 8192
-// slots took 48 us, half of it one CTA's reads of sixteen parts of 133 KB.)  An 8192-token prompt takes 540, 525, 524 and 532 us
-// with a PAD of 192, 256, 320 and 448; chunks of 500, 333 and 166 tokens over up to 7001 slots
-// 119, 111, 107 and 109.
+// slots took 48 us, half of it one CTA's reads of sixteen parts of 133 KB.)  An 8192-token prompt takes 534, 515, 499 and 495 us
+// with a PAD of 192, 256, 320 and 448, chunks of 500, 333 and 166 tokens over up to 7001 slots 112, 100, 93 and 97.
 constexpr int PAD = 320;
 // Shorter runs cost more in joining than they save: 128 tokens of 32/8 heads over 1024 slots take 23.0 us with two tiles at
 // least, 26.3 with four and 32.8 with eight, 64 tokens over 8192 slots 34.6, 33.3 and 36.4.
@@ -235,14 +236,20 @@ __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st16_issue(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_st8_issue(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Largest of three; NaN when one is (unlike fmaxf)
@@ -251,42 +258,29 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x for two x in [-126, 126] on the multiply-add pipe: x = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 leaves n
-// in the low bits), 2^f by a polynomial of degree 4 (largest relative error 2.6e-6, fitted to that by reweighted least
-// squares), n added to the exponent.
-__device__ __forceinline__ float2 ex2_poly(f32x2_t x) {
-  const f32x2_t big = pack_f32x2(12582912.f, 12582912.f), neg_big = pack_f32x2(-12582912.f, -12582912.f), minus = pack_f32x2(-1.f, -1.f);
-  const f32x2_t t = add_f32x2(x, big);
-  const f32x2_t f = fma_f32x2(add_f32x2(t, neg_big), minus, x);
-  f32x2_t y = fma_f32x2(f, pack_f32x2(0.009570101276040077f, 0.009570101276040077f), pack_f32x2(0.05591785907745361f, 0.05591785907745361f));
-  y = fma_f32x2(f, y, pack_f32x2(0.240247443318367f, 0.240247443318367f));
-  y = fma_f32x2(f, y, pack_f32x2(0.6931217908859253f, 0.6931217908859253f));
-  y = fma_f32x2(f, y, pack_f32x2(0.9999992847442627f, 0.9999992847442627f));
-  const float2 n = unpack_f32x2(t), r = unpack_f32x2(y);
-  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(r.y) + (__float_as_int(n.y) << 23)));
-}
-
-// The weights 2^(x * scale - base) of half a row's scores, as 16-bit pairs to tensor memory; returns their sum.  The unit
-// for 2^x makes 4 a clock and scheduler, as many clocks for both row tiles as their products take, and one warp does not
-// hide the rest behind it: FAST, one pair of three goes through the multiply-add pipe, whose polynomial takes no NaN or
-// infinity.  Measured, 128 columns by one warp a scheduler: 1269 clocks with none, 1093 with one of four, 1045 with
-// one of three, 1055 with one of two.
-constexpr int POLY_OF = 3;
-template <typename T, bool FAST>
-__device__ __forceinline__ float half_weights(const uint32_t* x, float scale, float base, uint32_t tp) {
+// Slots whose weights are handed over first: late enough that the thread that issues the products is not held up by the
+// rest, which the other row tile then waits for.  Measured, 8192-token prompt and chunks of 500, 333 and 166 tokens: 64
+// slots 521 and 107 us, 96 503 and 104, 112 494 and 101.
+constexpr int EARLY = 112;
+// The weights 2^(x * scale - base) of N scores of a row, as 16-bit pairs to tensor memory; returns their sum.  (With one pair
+// of four by a polynomial on the multiply-add pipe, to spare the unit for 2^x: prompts the same, chunks 99 us for 96.)
+template <typename T, int N>
+__device__ __forceinline__ float weights(const uint32_t* x, float scale, float base, uint32_t tp) {
   const f32x2_t scale2 = pack_f32x2(scale, scale), base2 = pack_f32x2(-base, -base);
   f32x2_t sum[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
-  uint32_t w[32];
+  static_assert(N % 32 == 0 || N % 32 == 16, "whole chunks");
+  uint32_t w[16];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < N / 2; ++i) {
     const f32x2_t v = fma_f32x2(pack_f32x2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, base2);
     float2 e = unpack_f32x2(v);
-    if (FAST && i % POLY_OF == POLY_OF - 1) e = ex2_poly(pack_f32x2(fmaxf(e.x, -126.f), fmaxf(e.y, -126.f)));
-    else e = make_float2(ex2(e.x), ex2(e.y));
+    e = make_float2(ex2(e.x), ex2(e.y));
     sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e.x, e.y));
-    w[i] = pack2<T>(e.x, e.y);
+    w[i % 16] = pack2<T>(e.x, e.y);
+    if (i % 16 == 15) tmem_st16_issue(tp + i - 15, w);
+    else if (i == N / 2 - 1) tmem_st8_issue(tp + i - 7, w);
   }
-  pre::tmem_st32(tp, w);
+  tmem_st_wait();
   const float2 s = unpack_f32x2(add_f32x2(sum[0], sum[1]));
   return s.x + s.y;
 }
@@ -508,7 +502,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
               if (!ok) break;
               pre::tc_fence_after();
 #pragma unroll
-              for (int k = h * 4; k < h * 4 + 4; ++k)
+              for (int k = h == 0 ? 0 : EARLY / 16; k < (h == 0 ? EARLY : TILE) / 16; ++k)
                 umma_f16_ta(tmem_base + TMEM_O + t * DIM, tmem_base + t * TILE + k * 8, bd + k * (2048 >> 4), j > j0 || k > 0, id_o);
             }
             if (!ok) break;
@@ -553,8 +547,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
           for (int c = 0; c < TILE; c += 32) tmem_ld32_issue(ts + c, x + c);
           tmem_ld_wait();
-          const bool clear = (j + 1) * TILE - 1 <= limit_all;
-          if (!clear) {
+          if ((j + 1) * TILE - 1 > limit_all) {
             const int last = limit - j * TILE;             // last visible column
 #pragma unroll
             for (int c = 0; c < TILE; ++c) x[c] = c <= last ? x[c] : 0xff800000u;
@@ -570,24 +563,20 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           for (int i = 0; i < 4; ++i) top[i] = max3_nan(top[i], __uint_as_float(x[TILE - 4 + i]), neg_inf());
           const float all_top = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], neg_inf());
           const float mx = all_top * p.scale_log2;         // (a NaN leaves the maximum alone and the weights are NaN)
-          // one vote a tile: some row's maximum has grown, or some score is not finite
-          bool fast = clear;
-          if (__any_sync(0xffffffffu, !(mx <= m + GROWTH) || !(mx > -3e38f))) {
-            fast = clear && __all_sync(0xffffffffu, fabsf(mx) < 3e38f);
-            if (__any_sync(0xffffffffu, mx > m + GROWTH)) {
-              const float a = mx > m ? ex2(m - mx) : 1.f;  // (m still minus infinity: zero)
-              m = fmaxf(m, mx);
-              l *= a;
-              if (j > j0) {
+          if (__any_sync(0xffffffffu, mx > m + GROWTH)) {
+            const float a = mx > m ? ex2(m - mx) : 1.f;    // (m still minus infinity: zero)
+            m = fmaxf(m, mx);
+            l *= a;
+            if (j > j0) {
 #pragma unroll
-                for (int c = 0; c < DIM; c += 16) {
-                  uint32_t o[16];
-                  csum::tmem_ld16(to + c, o);
+              for (int c = 0; c < DIM; c += 16) {
+                uint32_t o[16];
+                csum::tmem_ld16(to + c, o);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-                  tmem_st16(to + c, o);
-                }
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                tmem_st16_issue(to + c, o);
               }
+              tmem_st_wait();
             }
           }
           const float base = m == neg_inf() ? 0.f : m;
@@ -603,13 +592,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             }
             fence_proxy_async_smem();
           }
-          // The product with the first 64 slots' values starts while the other weights are made; it reads only rows of
-          // values that this warp's row tile has zeroed where need be (all four warps arrive for either half).
-          l += fast ? half_weights<T, true>(x, p.scale_log2, base, ts) : half_weights<T, false>(x, p.scale_log2, base, ts);
+          // The product with the first slots' values starts while the other weights are made; it reads only rows of
+          // values that this warp's row tile has zeroed where need be (all four warps arrive for either part).
+          l += weights<T, EARLY>(x, p.scale_log2, base, ts);
           pre::tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[2 * t]);
-          l += fast ? half_weights<T, true>(x + 64, p.scale_log2, base, ts + 32) : half_weights<T, false>(x + 64, p.scale_log2, base, ts + 32);
+          l += weights<T, TILE - EARLY>(x + EARLY, p.scale_log2, base, ts + EARLY / 2);
           pre::tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[2 * t + 1]);
