@@ -1,0 +1,53 @@
+"""Softmax weights of the attention on a paged cache: small ones that are all a row has to see."""
+
+import math
+
+import pytest
+import torch
+
+from tests import paged_helpers as R
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def cache(n_seqs, slots, heads, dim, dtype, fill):
+    """Sequences of `slots` slots, keys zero, values `fill`, pages of 64 in order."""
+    from zip_kernel_b200 import ops
+    cols = (slots + 63) // 64
+    k = torch.zeros(n_seqs * cols, heads, 64, dim, dtype=R.DT[dtype], device=DEV)
+    v = torch.full_like(k, fill)
+    table = torch.arange(n_seqs * cols, dtype=torch.int32, device=DEV).reshape(n_seqs, cols)
+    return ops.PagedKV(k, v, table), k, v
+
+
+def batch(n_seqs, new, slots):
+    return (torch.arange(n_seqs + 1, dtype=torch.int32, device=DEV) * new, torch.full((n_seqs,), slots, dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 4, 64])
+@pytest.mark.parametrize("gap", [12, 18, 20])
+def test_small_weights_are_all_there_is_to_see(dtype, dim, new, gap):
+    """One slot's score is `gap` above all others, its values are zero: the output is what the others, exp(-gap) each, add up
+    to.  Enough (sequence, head) pairs that most of them are not split."""
+    from zip_kernel_b200 import ops
+    B, G, n = 24, 8, 3000
+    kv, k, v = cache(B, n, G, dim, dtype, 8.0)
+    first = kv.block_table[:, 0].long()
+    k[first, :, 0, 0], v[first, :, 0] = gap / 2, 0.0
+    q = torch.zeros(B * new, 2 * G, dim, dtype=R.DT[dtype], device=DEV)
+    q[..., 0] = 2.0
+    cu, lengths = batch(B, new, n)
+    out, lse = ops.paged_attention_cuda(q, kv, cu, lengths, max_q_len=new, scale=1.0, return_lse=True)
+    others = torch.arange(n - new, n, dtype=torch.float64).repeat(B)          # slots that a row sees besides the first
+    w = others * math.exp(-gap)
+    u = torch.finfo(R.DT[dtype]).eps / 2
+    # half a step of the weights and of the output, the exponentials, the additions; an output below the normal range; and in
+    # the kernel for many rows weights below it: they are made 2^7 times as large, so half a step of 2^-24 is 2^-32 of a weight
+    rel = 2 * u + 2.0 ** -21 * (1 + gap) + (n + 16) * 2.0 ** -24
+    low = others * 8.0 * 2.0 ** -32 if dtype == "fp16" and 2 * new > 32 else torch.zeros_like(others)
+    want = (8.0 * w / (1 + w))[:, None, None].expand(out.shape)
+    R.assert_within(out, want, rel * want + low[:, None, None] + 2.0 ** -25, "out")
+    R.assert_within(lse, (gap + torch.log1p(w))[:, None].expand(lse.shape), 2.0 ** -20 * gap + (n + 16) * 2.0 ** -24, "lse")

@@ -3,8 +3,8 @@
 //   o[r] = sum_j p[r,j] v[j] / sum_j p[r,j],  p[r,j] = exp(scale q[r].k[j] - m[r]),  j up to the row's own slot,
 //
 // the running maximum m, the sum and o carried through one pass over the slots (o and the sum are multiplied by
-// exp(m_old - m_new) when the maximum grows).  A row = (new token, head of the group that shares the key/value head);
-// up to 16 rows fill the M side of an m16n8k16 product.
+// exp(m_old - m_new) when the maximum grows; fp16 weights are 2^15 times as large, see WEIGHT_SHIFT).  A row = (new token,
+// head of the group that shares the key/value head); up to 16 rows fill the M side of an m16n8k16 product.
 //
 // What bounds it: every key and value is read once from HBM, 2 * dim * 2 bytes for 4 * 16 * dim multiply-adds at most.
 // So the whole card must stream, whatever the number and lengths of the sequences: the 64-slot tiles of all (sequence,
@@ -312,7 +312,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         float top[MH];
         bool grown = false;
 #pragma unroll
-        for (int h = 0; h < MH; ++h) top[h] = m[h];
+        for (int h = 0; h < MH; ++h) top[h] = neg_inf();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -325,6 +325,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         for (int h = 0; h < MH; ++h) {
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+          top[h] = fmaxf(m[h], below_max(top[h], WEIGHT_SHIFT<T>));
           grown |= top[h] > m[h];
         }
         if (__any_sync(0xffffffffu, grown)) {

@@ -214,6 +214,12 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+// Weights are taken relative to a base below the maximum of their row, so that the largest is 2^SHIFT.  As fp16 relative to
+// the maximum itself, weights below 2^-25 would be lost, and in a long history with one slot far ahead whose values
+// are near zero they can be all there is to see.  Sums and outputs are larger by the same factor, which the quotient removes.
+// The subtraction rounds up: where a step of the maximum is coarse, no weight may exceed the type's range.
+template <typename T> constexpr float WEIGHT_SHIFT = std::is_same<T, __half>::value ? 15.f : 0.f;
+__device__ __forceinline__ float below_max(float top, float shift) { return __fadd_ru(top, -shift); }
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
 
 // cp.async.bulk.tensor of a 4-D box {element, slot, head, page}

@@ -11,8 +11,8 @@
 // in tensor memory, thread = row; the weights go back there as 16-bit pairs over the scores and are the A operand of the
 // second product, whose B operand is the value tile as it lands (slots x elements, read along the elements).  The output
 // stays in tensor memory; it is multiplied by exp(m_old - m_new) only when some row's maximum has grown by more than a
-// factor of 2^8, until when the weights are simply larger than one (2^8 at most: no worse rounded).  A weight is rounded
-// to the 16-bit type of the values, as the product demands: half a step of the output's own type.
+// factor of 2^8, until when the weights are simply larger (2^8 at most; fp16 weights are 2^7 times as large besides).  A
+// weight is rounded to the 16-bit type of the values, as the product demands: half a step of the output's own type.
 //
 // The order PV(j), S(j + 1) in the issuing thread makes one barrier do for two things: the scores of step j + 1 are
 // complete only after the product that reads the weights of step j and writes the output, so the softmax warps may
@@ -43,6 +43,8 @@ constexpr int REG_ISSUE = 88, REG_SOFTMAX = 208;
 static_assert(REG_ISSUE + 2 * REG_SOFTMAX <= 3 * 168, "the warpgroups share the registers of the launch");
 constexpr int TMEM_COLS = 512, TMEM_O = 256;
 constexpr float GROWTH = 8.f;                                // (log2) of a row's maximum before the output follows
+// Below the maximum by less than elsewhere, for the weights may grow by 2^GROWTH: fp16 loses what is below 2^-32 of the largest.
+template <typename T> constexpr float SHIFT = WEIGHT_SHIFT<T> > 0.f ? WEIGHT_SHIFT<T> - GROWTH : 0.f;
 
 enum : int { SITE_PPRE_EMPTY = 80, SITE_PPRE_Q, SITE_PPRE_K, SITE_PPRE_V, SITE_PPRE_P, SITE_PPRE_S, SITE_PPRE_VZERO, SITE_PPRE_O, SITE_PPRE_QEMPTY, SITE_PPRE_OEMPTY, SITE_PPRE_WORK, SITE_PPRE_WFREE };
 
@@ -562,8 +564,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
           for (int i = 0; i < 4; ++i) top[i] = max3_nan(top[i], __uint_as_float(x[TILE - 4 + i]), neg_inf());
           const float all_top = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], neg_inf());
-          const float mx = all_top * p.scale_log2;         // (a NaN leaves the maximum alone and the weights are NaN)
-          if (__any_sync(0xffffffffu, mx > m + GROWTH)) {
+          const float mx = below_max(all_top * p.scale_log2, SHIFT<T>);      // (a NaN leaves the maximum alone and the weights are NaN)
+          if (__any_sync(0xffffffffu, mx > __fadd_rd(m, GROWTH))) {
             const float a = mx > m ? ex2(m - mx) : 1.f;    // (m still minus infinity: zero)
             m = fmaxf(m, mx);
             l *= a;
