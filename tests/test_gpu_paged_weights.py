@@ -1,4 +1,5 @@
-"""Softmax weights of the attention on a paged cache: small ones that are all a row has to see."""
+"""Softmax weights of the attention on a paged cache: small ones that are all a row has to see, and
+those of scores so large that a step of them is more than a weight can follow."""
 
 import math
 
@@ -51,3 +52,23 @@ def test_small_weights_are_all_there_is_to_see(dtype, dim, new, gap):
     want = (8.0 * w / (1 + w))[:, None, None].expand(out.shape)
     R.assert_within(out, want, rel * want + low[:, None, None] + 2.0 ** -25, "out")
     R.assert_within(lse, (gap + torch.log1p(w))[:, None].expand(lse.shape), 2.0 ** -20 * gap + (n + 16) * 2.0 ** -24, "lse")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("new", [1, 40, 200])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("log2", list(range(18, 38)))
+def test_weights_of_equal_scores_are_equal_however_large_the_scores(dtype, new, sign, log2):
+    """All slots have the same key, scores up to 2^39: the output is the mean of the values, a constant."""
+    from zip_kernel_b200 import ops
+    B, G, n = 3, 2, 700
+    kv, k, v = cache(B, n, G, 128, dtype, 3.0)
+    a = log2 // 3                                                               # (12 at most: finite as fp16)
+    k[...], q = 0.0, torch.zeros(B * new, 2 * G, 128, dtype=R.DT[dtype], device=DEV)
+    k[..., 5], q[..., 5] = 1.3 * 2.0 ** a, sign * 1.7 * 2.0 ** a
+    scale = 1.1 * 2.0 ** (log2 - 2 * a)                                         # (products that round)
+    cu, lengths = batch(B, new, n)
+    out = ops.paged_attention_cuda(q, kv, cu, lengths, max_q_len=new, scale=scale)
+    # the weights are equal, but for the additions everything cancels; half a step of the weights and of the output
+    u = torch.finfo(R.DT[dtype]).eps / 2
+    R.assert_within(out, torch.full(out.shape, 3.0), 3.0 * (2 * u + (n + 16) * 2.0 ** -24), "out")

@@ -42,6 +42,9 @@ constexpr int WORKS = 4;                                     // units planned ah
 constexpr int REG_ISSUE = 88, REG_SOFTMAX = 208;
 static_assert(REG_ISSUE + 2 * REG_SOFTMAX <= 3 * 168, "the warpgroups share the registers of the launch");
 constexpr int TMEM_COLS = 512, TMEM_O = 256;
+// Scores (log2) from which on their product with the scale is rounded before the maximum is taken off: a weight is made with
+// one rounding for both, the maximum is a rounded product, and from here on the two may differ by more than half a step of 2.
+constexpr float HUGE_SCORE = 4194304.f;
 constexpr float GROWTH = 8.f;                                // (log2) of a row's maximum before the output follows
 // Below the maximum by less than elsewhere, for the weights may grow by 2^GROWTH: fp16 loses what is below 2^-32 of the largest.
 template <typename T> constexpr float SHIFT = WEIGHT_SHIFT<T> > 0.f ? WEIGHT_SHIFT<T> - GROWTH : 0.f;
@@ -564,8 +567,16 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
           for (int i = 0; i < 4; ++i) top[i] = max3_nan(top[i], __uint_as_float(x[TILE - 4 + i]), neg_inf());
           const float all_top = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], neg_inf());
-          const float mx = below_max(all_top * p.scale_log2, SHIFT<T>);      // (a NaN leaves the maximum alone and the weights are NaN)
-          if (__any_sync(0xffffffffu, mx > __fadd_rd(m, GROWTH))) {
+          const float scaled = all_top * p.scale_log2;     // (a NaN leaves the maximum alone and the weights are NaN)
+          const float mx = below_max(scaled, SHIFT<T>);
+          float scale = p.scale_log2;
+          const bool huge = fabsf(scaled) > HUGE_SCORE && scaled != neg_inf();
+          if (__any_sync(0xffffffffu, mx > __fadd_rd(m, GROWTH) || huge)) {
+            if (__any_sync(0xffffffffu, huge)) {
+#pragma unroll
+              for (int c = 0; c < TILE; ++c) x[c] = __float_as_uint(__fmul_rn(__uint_as_float(x[c]), scale));
+              scale = 1.f;
+            }
             const float a = mx > m ? ex2(m - mx) : 1.f;    // (m still minus infinity: zero)
             m = fmaxf(m, mx);
             l *= a;
@@ -596,11 +607,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           }
           // The product with the first slots' values starts while the other weights are made; it reads only rows of
           // values that this warp's row tile has zeroed where need be (all four warps arrive for either part).
-          l += weights<T, EARLY>(x, p.scale_log2, base, ts);
+          l += weights<T, EARLY>(x, scale, base, ts);
           pre::tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[2 * t]);
-          l += weights<T, TILE - EARLY>(x + EARLY, p.scale_log2, base, ts + EARLY / 2);
+          l += weights<T, TILE - EARLY>(x + EARLY, scale, base, ts + EARLY / 2);
           pre::tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[2 * t + 1]);
