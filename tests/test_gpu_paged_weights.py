@@ -72,3 +72,26 @@ def test_weights_of_equal_scores_are_equal_however_large_the_scores(dtype, new, 
     # the weights are equal, but for the additions everything cancels; half a step of the weights and of the output
     u = torch.finfo(R.DT[dtype]).eps / 2
     R.assert_within(out, torch.full(out.shape, 3.0), 3.0 * (2 * u + (n + 16) * 2.0 ** -24), "out")
+
+
+@pytest.mark.parametrize("news,lens,heads,kv_heads,dim,page", [
+    ([1, 1, 1, 1], [1, 5, 17, 64], 32, 8, 128, 16),
+    ([1, 1], [40, 7], 16, 1, 64, 48),
+    ([3, 1, 4], [3, 30, 60], 8, 2, 128, 16),
+    ([8], [50], 4, 1, 64, 32),
+])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_weights_of_few_rows_are_not_rounded_to_the_type(news, lens, heads, kv_heads, dim, page, dtype):
+    """One rounding, that of the output: a weight enters as two terms, which leave (half a step)^2 of it.  Queries and keys are
+    small whole numbers, their products and sums exact."""
+    from zip_kernel_b200 import ops
+    c = R.Case(news, lens, heads, kv_heads, dim, page, dtype, seed=23)
+    g = torch.Generator().manual_seed(24)
+    c.q = torch.randint(-2, 3, c.q.shape, generator=g).to(c.dt)
+    c.k = torch.where(torch.isnan(c.k), c.k, torch.randint(-2, 3, c.k.shape, generator=g).to(c.dt))
+    ref, _, amp, mag = R.attention_ref(c)
+    out = ops.paged_attention_cuda(c.q.to(DEV), c.kv(), c.cu.to(DEV), c.lengths.to(DEV), max_q_len=max(news))
+    u = torch.finfo(c.dt).eps / 2
+    # the scale's rounding and the exponentials, the additions
+    rel = u * u + 2.0 ** -21 * (1 + mag) + (max(lens) + 16) * 2.0 ** -24
+    R.assert_within(out, ref, u * ref.abs() + 1.01 * rel[..., None] * (amp + ref.abs()) + 2.0 ** -25, "out")
