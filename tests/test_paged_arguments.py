@@ -1,0 +1,29 @@
+"""Checks of the paged-cache operators that look at shapes and strides alone: no GPU."""
+
+import pytest
+import torch
+
+
+def table(rows, cols, strides=None):
+    t = torch.zeros(4096, dtype=torch.int32)
+    return t[:rows * cols].view(rows, cols) if strides is None else t.as_strided((rows, cols), strides)
+
+
+@pytest.mark.parametrize("t,stride", [
+    (table(4, 6), 6), (table(4, 6, (9, 1)), 9), (table(1, 6, (0, 1)), 6), (table(0, 6), 6), (table(4, 1, (1, 7)), 1), (table(4, 1, (5, 0)), 5),
+    (table(4, 6)[:, :0], 6), (table(4, 0), 1), (table(3, 6).expand(3, 6), 6), (table(1, 6).expand(1, 6), 6),
+])
+def test_row_stride_of_a_block_table(t, stride):
+    from zip_kernel_b200 import paged_ops
+    assert paged_ops._table_stride(t) >= t.shape[1] and (t.shape[0] < 2 or paged_ops._table_stride(t) == stride)
+
+
+@pytest.mark.parametrize("t", [
+    table(1, 6).expand(4, 6),                               # one row for all sequences: stride 0
+    table(4, 6, (5, 1)), table(2, 6, (1, 1)),               # rows that overlap
+    table(4, 6, (12, 2)), table(6, 4).T, table(4, 1).expand(4, 3),
+])
+def test_block_tables_whose_rows_are_not_apart_are_refused(t):
+    from zip_kernel_b200 import paged_ops
+    with pytest.raises(ValueError, match="apart"):
+        paged_ops._table_stride(t)

@@ -40,6 +40,14 @@ def _strides(t: torch.Tensor):
     return out[::-1]
 
 
+def _table_stride(table: torch.Tensor) -> int:
+    """Row stride of a block table whose rows lie apart."""
+    (rows, cols), (row, col) = table.shape, _strides(table)
+    if (cols > 1 and col != 1) or (rows > 1 and row < cols):
+        raise ValueError(f"the rows of block_table must be contiguous and apart (an expanded one: .contiguous()), got strides {tuple(table.stride())}")
+    return max(row, cols)
+
+
 class PagedKV:
     """Key and value pages ``(n_pages, n_kv_heads, page_size, head_dim)`` fp16 or bf16 and the block table
     ``(B, max_pages)`` int32 of the sequences that use them.  The tensors are referred to, not copied; any strides over
@@ -62,13 +70,11 @@ class PagedKV:
             raise ValueError(f"page_size must be a positive multiple of 16, got {page}")
         if n_pages < 1 or n_kv < 1:
             raise ValueError("there must be a page and a head")
-        ks, vs, ts = _strides(k_pages), _strides(v_pages), _strides(block_table)
+        ks, vs, ts = _strides(k_pages), _strides(v_pages), _table_stride(block_table)
         for name, t, st in (("k_pages", k_pages, ks), ("v_pages", v_pages, vs)):
             if st[3] != 1 or any(s <= 0 or s % 8 for s in st[:3]) or t.data_ptr() % 16:
                 raise ValueError(f"{name}: rows must be contiguous, strides positive multiples of 8 elements, the address of 16 bytes; "
                                  f"got strides {tuple(t.stride())}")
-        if block_table.shape[1] > 1 and ts[1] != 1:
-            raise ValueError("the rows of block_table must be contiguous")
         self.k_pages, self.v_pages, self.block_table = k_pages, v_pages, block_table
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = (int(x) for x in k_pages.shape)
         self.n_seqs, self.max_pages = (int(x) for x in block_table.shape)
@@ -78,7 +84,7 @@ class PagedKV:
             raise ValueError(f"a sequence of {self.max_pages} pages of {self.page_size} slots is too long")
         self._arg = _lib.PagedKVArg(
             k_pages.data_ptr(), v_pages.data_ptr(), (ctypes.c_longlong * 3)(*ks[:3]), (ctypes.c_longlong * 3)(*vs[:3]),
-            block_table.data_ptr(), max(ts[0], self.max_pages), self.n_pages, self.page_size, self.n_kv_heads, self.head_dim,
+            block_table.data_ptr(), ts, self.n_pages, self.page_size, self.n_kv_heads, self.head_dim,
             self.n_seqs, self.max_pages, DTYPES[self.dtype])
         self._ptr = ctypes.addressof(self._arg)
         self._cu_shape, self._len_shape = (self.n_seqs + 1,), (self.n_seqs,)
