@@ -1,0 +1,56 @@
+"""Calls from several host threads of one process."""
+
+import pytest
+import torch
+
+from tests import paged_helpers as R
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def in_threads(*jobs):
+    """Runs the jobs at once, on the default stream of each thread, and passes on the first exception."""
+    import threading
+    errors, start = [], threading.Barrier(len(jobs))
+
+    def work(job):
+        try:
+            start.wait()
+            job()
+        except BaseException as e:                                           # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    if errors:
+        raise errors[0]
+
+
+def test_first_cuda_call_of_a_thread():
+    """Threads that have no current context yet: all that the calls need is there, so nothing else makes one current."""
+    from zip_kernel_b200 import ops, synth
+    c = R.Case([1, 40], [50, 60], 8, 2, 128, 16, "fp16", seed=30)
+    kv, q, cu, n = c.kv(), c.q.to(DEV), c.cu.to(DEV), c.lengths.to(DEV)
+    want, lse = ops.paged_attention_cuda(q, kv, cu, n, return_lse=True)
+    want_sums = ops.cache_weight_sums_cuda(q, kv, cu, n, lse, torch.zeros(2, 2, kv.max_slots, device=DEV))
+    out, total = torch.zeros_like(want), torch.zeros_like(want_sums)
+    X = synth.make_activations(300, 512, seed=1).to(DEV)
+    W = [synth.make_container(256, 512, 0.2, seed=2).to(DEV) for _ in range(2)]
+    xs4, sx, sumx = ops.activation_quant_cuda(X, W[0].perm)
+    codes, group_sums = ops.expand_activations_cuda(xs4, sumx)
+
+    def linear(w):
+        return ops.fused_dense_sparse_expanded_cuda(w.W_low_packed, w.W_high_blocks_packed, w.hp_row_offsets, w.hp_col_indices, codes,
+                                                    group_sums, w.scale_u4, w.zero_u4, sx, 256, 512)
+
+    want_y, y = linear(W[0]), []
+    torch.cuda.synchronize()
+    in_threads(lambda: ops.paged_attention_cuda(q, kv, cu, n, out=out))
+    in_threads(lambda: ops.cache_weight_sums_cuda(q, kv, cu, n, lse, total))
+    in_threads(lambda: y.append(linear(W[1])))               # (weights at addresses that no call has seen)
+    assert torch.equal(out, want) and torch.equal(total, want_sums) and torch.equal(y[0], want_y)

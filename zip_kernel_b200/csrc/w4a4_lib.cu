@@ -155,6 +155,17 @@ int current_device(DeviceInfo** out) {
   return W4A4_OK;
 }
 
+// Encoding a map is a call of the driver and needs a current context, which a thread that has made no call of the runtime
+// but asking for its device does not have yet.
+template <typename... Args>
+CUresult encode_map(Args... args) {
+  CUresult r = g_encode(args...);
+  if (r != CUDA_ERROR_INVALID_CONTEXT) return r;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return r;
+  return g_encode(args...);
+}
+
 // 2-D byte tensor map: `rows` rows of `row_bytes` bytes (pitch = row_bytes), box
 // box_bytes x box_rows.  Out-of-range rows read as zero.  A map depends only on the
 // address and the geometry, so encoded maps are kept (weights are called with the
@@ -197,9 +208,9 @@ int make_map(CUtensorMap* m, const void* ptr, uint64_t row_bytes, uint64_t rows,
   cuuint64_t strides[1] = {row_bytes};
   cuuint32_t box[2] = {box_bytes, box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(W4A4_ERR_LAUNCH, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   std::lock_guard<std::mutex> lock(g_mutex);
   if (g_maps.size() >= MAP_CACHE_LIMIT) g_maps.clear();
