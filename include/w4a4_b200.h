@@ -364,7 +364,8 @@ int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long l
  * beyond the length they may hold anything.  max_q_len: no sequence has more new tokens.
  * workspace: w4a4_paged_attention_workspace_bytes (0: an argument is bad), 16-byte aligned; its first
  * W4A4_ATTENTION_STATE_BYTES must be zero before the first call and are zero again after each; calls that share it
- * must be ordered on one stream.  It is not the workspace of the linears. */
+ * must be ordered on one stream, from whatever threads: the launches of a call stay together there.  It is not the
+ * workspace of the linears. */
 #define W4A4_ATTENTION_STATE_BYTES 4096
 size_t w4a4_paged_attention_workspace_bytes(const w4a4_paged_kv* cache, int T, int n_heads, int max_q_len);
 int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,

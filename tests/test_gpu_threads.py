@@ -54,3 +54,22 @@ def test_first_cuda_call_of_a_thread():
     in_threads(lambda: ops.cache_weight_sums_cuda(q, kv, cu, n, lse, total))
     in_threads(lambda: y.append(linear(W[1])))               # (weights at addresses that no call has seen)
     assert torch.equal(out, want) and torch.equal(total, want_sums) and torch.equal(y[0], want_y)
+
+
+def test_attention_of_threads_that_share_a_stream():
+    """Prompts whose units are cut (a join after the kernel), a mixed batch and decode steps, issued by four threads on one
+    stream with one workspace: the bits that each gives alone."""
+    from zip_kernel_b200 import _lib, ops
+    cases = [R.Case([64], [3000], 8, 2, 128, 16, "fp16", seed=31), R.Case([200, 3, 90], [900, 40, 2000], 8, 2, 128, 16, "fp16", seed=32),
+             R.Case([1] * 9, [700 - 60 * b for b in range(9)], 8, 2, 128, 16, "fp16", seed=33), R.Case([33], [1500], 8, 2, 64, 32, "bf16", seed=34)]
+    args = [(c.q.to(DEV), c.kv(), c.cu.to(DEV), c.lengths.to(DEV)) for c in cases]
+    want = [ops.paged_attention_cuda(*a, max_q_len=max(c.news)) for a, c in zip(args, cases)]
+    got = [[] for _ in cases]
+
+    def job(i):
+        return lambda: got[i].extend(ops.paged_attention_cuda(*args[i], max_q_len=max(cases[i].news)) for _ in range(150))
+
+    in_threads(*(job(i) for i in range(len(cases))))
+    for w, outs in zip(want, got):
+        assert len(outs) == 150 and all(torch.equal(o, w) for o in outs)
+    assert _lib.device_error(DEV) == 0

@@ -298,6 +298,7 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
     return fail(W4A4_ERR_WORKSPACE, "workspace of %zu bytes required, got %zu", plan.total, workspace_bytes);
   if (!aligned(workspace, 16)) return fail(W4A4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
   if (dev->sm_count > pdec::MAX_RUNS) return fail(W4A4_ERR_UNSUPPORTED, "%d SMs", dev->sm_count);
+  std::lock_guard<std::recursive_mutex> together(dev->launches);
   char* ws = static_cast<char*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool d128 = cache->head_dim == 128;

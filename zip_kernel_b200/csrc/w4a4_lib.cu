@@ -56,6 +56,9 @@ inline size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 struct DeviceInfo {
   int sm_count = 0;
   bool attrs_set = false;
+  // Held while a call issues several launches that hand data on through a workspace: another thread's call on the same
+  // stream and workspace must not come in between.
+  std::recursive_mutex launches;
 };
 std::mutex g_mutex;
 DeviceInfo g_dev[64];
