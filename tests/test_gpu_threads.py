@@ -73,3 +73,20 @@ def test_attention_of_threads_that_share_a_stream():
     for w, outs in zip(want, got):
         assert len(outs) == 150 and all(torch.equal(o, w) for o in outs)
     assert _lib.device_error(DEV) == 0
+
+
+def test_linears_of_threads_that_share_a_stream():
+    """Quantisation and GEMM of four threads on one stream with one workspace, few tokens and many: the bits that each gives alone."""
+    from zip_kernel_b200 import _lib, synth, v9_linear
+    W = synth.make_container(512, 1024, 0.2, seed=3).to(DEV)
+    X = [synth.make_activations(t, 1024, seed=40 + t).to(DEV) for t in (4, 40, 300, 301)]
+    want = [v9_linear.v9_linear_forward(x, W) for x in X]
+    got = [[] for _ in X]
+
+    def job(i):
+        return lambda: got[i].extend(v9_linear.v9_linear_forward(X[i], W) for _ in range(150))
+
+    in_threads(*(job(i) for i in range(len(X))))
+    for w, outs in zip(want, got):
+        assert len(outs) == 150 and all(torch.equal(o, w) for o in outs)
+    assert _lib.device_error(DEV) == 0

@@ -161,7 +161,8 @@ def on_device(device):
 
 # ---------------------------------------------------------------------------
 # workspace cache: one scratch buffer per (device, stream), grown on
-# demand.  Calls issued on one stream are ordered, so they can share scratch.
+# demand.  Calls issued on one stream are ordered, so they can share scratch; the
+# library keeps the launches of a call together when threads share a stream.
 #
 # A captured CUDA graph bakes the scratch address into its kernel nodes, so a
 # graph must own the scratch it was captured with: a buffer from the shared

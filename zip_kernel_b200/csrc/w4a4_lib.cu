@@ -755,6 +755,7 @@ int run_gemm(GemmArgs& a) {
     return fail(W4A4_ERR_UNSUPPORTED, "tensor-core path does not support T=%d K=%d N=%d", a.T, a.K, a.N);
   if (!aligned(a.W_low_prep, 16) || !aligned(a.W_high_prep, 16))
     return fail(W4A4_ERR_ALIGNMENT, "weight pointers must be 16-byte aligned");
+  std::lock_guard<std::recursive_mutex> together(dev->launches);
   // e4m3 codes exist only for the tensor-core kernel: such a call goes there whatever the token count
   if ((a.XE != nullptr && a.xe_fmt != 0) || ((a.acc_dump || a.acc_hi_dump) && (a.flags & W4A4_FLAG_CODES_E4M3_PACKED))) {
     if (a.flags & W4A4_FLAG_FORCE_STREAM) return fail(W4A4_ERR_BAD_ARG, "the streaming path reads s8 expanded codes");
@@ -1261,6 +1262,7 @@ int w4a4_fused_quant_dense_sparse_prepared(const void* X, long long ldx, const i
                                            true, dev->sm_count).codes
                     : W4A4_CODES_S8;
   a.widen = tensor && !has_prepared(a) && a.xe_fmt == W4A4_CODES_E4M3;
+  std::lock_guard<std::recursive_mutex> together(dev->launches);
   rc = launch_quant(X, ldx, perm, nullptr, ws + wl.scale_x, nullptr, ws + wl.xe, reinterpret_cast<float*>(ws + wl.sumxf),
                     T, K, s, dev->sm_count, a.xe_fmt);
   if (rc) return rc;
@@ -1322,6 +1324,7 @@ int w4a4_fused_dense_sparse_noalloc(const void* W_low, const void* W_high, const
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   char* xe = static_cast<char*>(scratch);
   float* sums = reinterpret_cast<float*>(xe + NOALLOC_XE_BYTES);
+  std::lock_guard<std::recursive_mutex> together(dev->launches);
   // The array keeps whatever the previous call left.  The codes of the T live
   // tokens are overwritten below and rows past T are never read; the group sums of
   // the token tile are cleared so that no stale lane of an earlier call is read.
