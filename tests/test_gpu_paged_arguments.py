@@ -23,3 +23,17 @@ def test_a_block_table_that_sequences_share_is_refused():
     out = ops.paged_attention_cuda(q[:1].repeat(2, 1, 1), shared, cu, n, max_q_len=1)
     ref, _, amp, mag = R.attention_ref(c)
     R.assert_within(out, ref[:1].expand(2, -1, -1), R.attention_tolerance(c, ref, amp, mag)[:1].expand(2, -1, -1), "out")
+
+
+def test_sequences_without_any_page_need_no_earlier_call():
+    """A block table without columns has no address; the workspace is this call's own."""
+    from zip_kernel_b200 import _lib, ops
+    c = R.Case([2, 1], [4, 7], 8, 2, 128, 16, "fp16", seed=20)
+    full, cu, n, q = c.kv(), c.cu.to(DEV), torch.zeros(2, dtype=torch.int32, device=DEV), c.q.to(DEV)
+    kv = ops.PagedKV(full.k_pages, full.v_pages, torch.zeros(2, 0, dtype=torch.int32, device=DEV))
+    for q_len in (2, 1):
+        with _lib.use_workspace(_lib.WorkspaceHolder()):
+            out, lse = ops.paged_attention_cuda(q, kv, cu if q_len == 2 else torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV), n,
+                                                max_q_len=q_len, return_lse=True)
+        assert (out[:q_len + 1] == 0).all() and (lse[:q_len + 1] == float("-inf")).all()
+    assert _lib.device_error(DEV) == 0

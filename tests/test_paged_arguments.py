@@ -27,3 +27,21 @@ def test_block_tables_whose_rows_are_not_apart_are_refused(t):
     from zip_kernel_b200 import paged_ops
     with pytest.raises(ValueError, match="apart"):
         paged_ops._table_stride(t)
+
+
+def test_workspace_query_takes_a_cache_without_pages():
+    """It may fail for want of a device, not of a block table; a bad argument is named."""
+    from tests.test_paged_refusals import arg
+    import ctypes
+    from zip_kernel_b200 import _lib
+    L = _lib.load()
+
+    def query(kv, T=3, n_heads=32, max_q=1):
+        got = L.w4a4_paged_attention_workspace_bytes(ctypes.addressof(kv), T, n_heads, max_q)
+        return got, L.w4a4_last_error().decode()
+
+    got, why = query(arg(block_table=None, max_pages=0))
+    assert got > 0 or "cuda" in why
+    for kw, word in ((dict(T=-1), "negative"), (dict(n_heads=12), "multiple"), (dict(max_q=-1), "max_q_len")):
+        got, why = query(arg(), **kw)
+        assert got == 0 and word in why

@@ -236,7 +236,10 @@ def workspace(device: torch.device, T: int, K: int, N: int, nnz: int) -> torch.T
 
 def attention_workspace(kv, T: int, n_heads: int, max_q_len: int, stream: int) -> torch.Tensor:
     """Scratch of the attention on a paged cache: apart from the linears' because its counters start, and end, as zeros."""
-    need = int(load().w4a4_paged_attention_workspace_bytes(kv._ptr, T, n_heads, max_q_len))
+    lib = load()
+    need = int(lib.w4a4_paged_attention_workspace_bytes(kv._ptr, T, n_heads, max_q_len))
+    if need == 0:
+        raise RuntimeError("the size of the attention workspace: " + (lib.w4a4_last_error() or b"").decode())
     key = (kv.device.index, stream, "attention")
     holder = getattr(_tls, "holder", None)
     if holder is not None:

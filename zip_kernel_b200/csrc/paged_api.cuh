@@ -70,10 +70,16 @@ int check_rows(const char* what, const void* ptr, long long tok, long long head,
   return W4A4_OK;
 }
 
-int check_seqs(const w4a4_paged_kv* c, const int32_t* cu, const int32_t* lengths, int T, int n_heads) {
+int check_sizes(const w4a4_paged_kv* c, int T, int n_heads) {
   CHECK_ARG(T >= 0, "T must not be negative, got %d", T);
   CHECK_ARG(n_heads >= 1 && n_heads % c->n_kv_heads == 0, "n_heads (%d) must be a positive multiple of n_kv_heads (%d)", n_heads,
             c->n_kv_heads);
+  return W4A4_OK;
+}
+
+int check_seqs(const w4a4_paged_kv* c, const int32_t* cu, const int32_t* lengths, int T, int n_heads) {
+  const int rc = check_sizes(c, T, n_heads);
+  if (rc) return rc;
   CHECK_ARG(c->n_seqs == 0 || (cu && lengths), "cu_seqlens or lengths is NULL");
   if (!aligned(cu, 4) || !aligned(lengths, 4)) return fail(W4A4_ERR_ALIGNMENT, "cu_seqlens and lengths must be 4-byte aligned");
   return W4A4_OK;
@@ -268,7 +274,11 @@ int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long l
 
 size_t w4a4_paged_attention_workspace_bytes(const w4a4_paged_kv* cache, int T, int n_heads, int max_q_len) {
   begin_call();
-  if (check_cache(cache) || check_seqs(cache, cache->block_table, cache->block_table, T, n_heads) || max_q_len < 0) return 0;
+  if (check_cache(cache) || check_sizes(cache, T, n_heads)) return 0;
+  if (max_q_len < 0) {
+    fail(W4A4_ERR_BAD_ARG, "max_q_len must not be negative, got %d", max_q_len);
+    return 0;
+  }
   DeviceInfo* dev = nullptr;
   if (current_device(&dev)) return 0;
   return attn_plan(cache, T, n_heads, max_q_len < T ? max_q_len : T, dev->sm_count).total;
