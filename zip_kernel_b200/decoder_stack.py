@@ -136,7 +136,8 @@ class DecoderStack:
         self.v_cache = torch.zeros_like(self.k_cache)
 
     # ---- the same on the paged cache: x holds the S newest tokens of every sequence, whose slots `cu` and the lengths give
-    def _layer_paged(self, li: int, x: torch.Tensor, cu: torch.Tensor) -> torch.Tensor:
+    # (the attention weight of the last `counted` of them is added up)
+    def _layer_paged(self, li: int, x: torch.Tensor, cu: torch.Tensor, counted: int = 0) -> torch.Tensor:
         cfg, L, cache, kv = self.cfg, self.layers[li], self.cache, self.cache.layer(li)
         B, S, _ = x.shape
         if self.fused_seams:
@@ -145,14 +146,14 @@ class DecoderStack:
             qkv = v9_linear_forward(rms_norm(x, L.norm1, cfg.rms_eps), L.qkv)
         q = ops.qkv_rope_cache_cuda(qkv.view(B * S, -1), kv, cu, cache.lengths, self.cos32, self.sin32, q_norm=self.q_norm,
                                     k_norm=self.k_norm, eps=cfg.rms_eps, interleaved=True, offsets=cache.offsets)
-        if cache.sums is None:
+        if cache.sums is None or counted == 0:
             att = ops.paged_attention_cuda(q, kv, cu, cache.lengths, max_q_len=S)
         else:
             att, lse = ops.paged_attention_cuda(q, kv, cu, cache.lengths, max_q_len=S, return_lse=True)
-            n = min(S, self.WEIGHT_WINDOW)
-            if n == S:
+            if counted == S:
                 cache.add_weights(li, q, lse, cu, S)
             else:
+                n = counted
                 last = q.view(B, S, cfg.n_heads, cfg.head_dim)[:, -n:].reshape(B * n, cfg.n_heads, cfg.head_dim)
                 cache.add_weights(li, last, lse.view(B, S, -1)[:, -n:].reshape(B * n, -1), cache.cu_seqlens(n), n)
         x = x + v9_linear_forward(att.view(B, S, cfg.n_heads * cfg.head_dim), L.o)
@@ -207,10 +208,12 @@ class DecoderStack:
         if self.cache is not None:
             for c0 in range(0, S, chunk or S):
                 part = tokens[:, c0:c0 + (chunk or S)]
-                cu = self.cache.advance(part.shape[1])
+                n = part.shape[1]
+                counted = max(0, min(n, c0 + n - (S - self.WEIGHT_WINDOW)))      # those among the prompt's last ones
+                cu = self.cache.advance(n)
                 x = self.embed[part]
                 for li in range(self.cfg.n_layers):
-                    x = self._layer_paged(li, x, cu)
+                    x = self._layer_paged(li, x, cu, counted)
         else:
             x = self.embed[tokens]
             for li in range(self.cfg.n_layers):
@@ -231,7 +234,7 @@ class DecoderStack:
         if self.cache is not None:
             cu = self.cache.advance(1)
             for li in range(self.cfg.n_layers):
-                x = self._layer_paged(li, x, cu)
+                x = self._layer_paged(li, x, cu, 1)
         else:
             for li in range(self.cfg.n_layers):
                 x = self._layer(li, x, pos, 1, attend_len)
