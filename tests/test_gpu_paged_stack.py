@@ -40,6 +40,23 @@ def test_weight_of_a_prompt_in_chunks_is_that_of_its_last_tokens(S):
         assert ((first - whole).abs() <= 0.05 * whole).all(), chunk
 
 
+def test_sums_after_a_run_do_not_depend_on_the_graph(monkeypatch):
+    from zip_kernel_b200 import decoder_stack as ds
+    made = []
+
+    class Recorded(ds.DecoderStack):
+        def __init__(self, *a, **kw):
+            super().__init__(*a, **kw)
+            made.append(self)
+
+    monkeypatch.setattr(ds, "DecoderStack", Recorded)
+    for graph in (True, False):
+        ds.run(small_cfg(), batch=2, prefill_len=40, decode_steps=6, device=DEV, use_graph=graph, seed=3, paged=True, chunk=24, evict=12)
+    a, b = (s.cache for s in made)
+    assert torch.equal(a.sums, b.sums) and torch.equal(a.lengths, b.lengths) and torch.equal(a.offsets, b.offsets)
+    assert not a.sums[..., 12:].any()                       # nothing is added once the histories are cut
+
+
 def test_the_stack_hands_the_operators_the_right_slots_and_positions(monkeypatch):
     """Chunks of a prompt, decode steps, an eviction, decode steps: rotation, cache write and attention of every layer against 64
     bits, at slots and positions that the test counts itself."""

@@ -101,6 +101,7 @@ class DecoderStack:
     """Weights, KV cache and the two phases (prefill of a prompt batch, one decode step)."""
 
     WEIGHT_WINDOW = 32             # last prompt tokens whose attention weight counts for an eviction
+    weigh_decode = True            # with track_weights, a decode step's counts too; off once no eviction is to follow
 
     def __init__(self, cfg: StackConfig, batch: int, max_len: int, device, seed: int = 0, prepared: bool = True,
                  fused_seams: bool = True, paged: bool = False, track_weights: bool = False):
@@ -234,7 +235,7 @@ class DecoderStack:
         if self.cache is not None:
             cu = self.cache.advance(1)
             for li in range(self.cfg.n_layers):
-                x = self._layer_paged(li, x, cu, 1)
+                x = self._layer_paged(li, x, cu, 1 if self.weigh_decode else 0)
         else:
             for li in range(self.cfg.n_layers):
                 x = self._layer(li, x, pos, 1, attend_len)
@@ -264,6 +265,7 @@ def run(cfg: StackConfig, batch: int, prefill_len: int, decode_steps: int, devic
         t_prefill = time.perf_counter() - t0
         if evict:
             stack.cache.evict(evict, n_sink=min(4, evict // 2), n_recent=min(stack.WEIGHT_WINDOW, evict // 2))
+            stack.weigh_decode = False
 
         pos = torch.tensor([prefill_len], dtype=torch.int64, device=device)
         tok = nxt.clone()
