@@ -375,7 +375,8 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
 
 /* Adds to sums[b, g, j] the attention weight that slot j of sequence b has received from the call's new tokens:
  * sum over the new tokens i that see j and the heads h of group g of exp(scale * q[i, h] . k[j] - lse[i, h]), lse from
- * w4a4_paged_attention; at most 128 heads share a key/value head.  sums: float, row strides in elements, at least
+ * w4a4_paged_attention; at most 128 heads share a key/value head, and a table's 128-slot tiles times the 128-row tiles of
+ * max_q_len tokens are at most 2^30.  sums: float, row strides in elements, at least
  * max_pages * page_size floats a row; slots beyond a sequence's length are not touched.  _fresh: sums holds nothing yet;
  * the same as on zeros, every slot of every row is written (T and max_q_len must be positive then). */
 int w4a4_cache_weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_stride, long long q_head_stride,

@@ -45,3 +45,13 @@ def test_workspace_query_takes_a_cache_without_pages():
     for kw, word in ((dict(T=-1), "negative"), (dict(n_heads=12), "multiple"), (dict(max_q=-1), "max_q_len")):
         got, why = query(arg(), **kw)
         assert got == 0 and word in why
+
+
+def test_weight_sums_of_more_steps_than_are_counted_are_refused():
+    """2^24 slot tiles; a row tile of 8 heads holds 16 tokens, so 2048 tokens make 128 of them: 2^31 steps of a unit."""
+    from tests.test_paged_refusals import UNSUPPORTED, arg, sums
+    from zip_kernel_b200 import _lib
+    slots = ((1 << 27) - 80) * 16
+    kv = arg(max_pages=slots // 16, table_stride=slots // 16)
+    big = dict(seq=8 * slots, head=slots, n_heads=64, T=1 << 20)
+    assert sums(kv, max_q=2048, **big) == UNSUPPORTED and "too many" in _lib.load().w4a4_last_error().decode()

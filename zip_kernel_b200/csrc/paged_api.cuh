@@ -173,10 +173,17 @@ int weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_strid
   if (rc) return rc;
   CHECK_ARG(lse && sums, "lse or sums is NULL");
   if (!aligned(lse, 4) || !aligned(sums, 4)) return fail(W4A4_ERR_ALIGNMENT, "lse and sums must be 4-byte aligned");
+  max_q_len = max_q_len < T ? max_q_len : T;
+  // the narrowest product that takes all rows of the longest sequence, 128 at most
+  const long long rows = (long long)max_q_len * group;
+  const int cols = rows >= csum::MAX_COLS ? csum::MAX_COLS : (int)((rows + 15) / 16 * 16);
+  // steps of a unit are counted in 32 bits
+  const long long row_tiles = ((long long)max_q_len + cols / group - 1) / (cols / group);
+  if ((slots + csum::TILE - 1) / csum::TILE * row_tiles > (1LL << 30))
+    return fail(W4A4_ERR_UNSUPPORTED, "%d new tokens over %lld slots are too many for one call", max_q_len, slots);
   DeviceInfo* dev = nullptr;
   rc = current_device(&dev);
   if (rc) return rc;
-  max_q_len = max_q_len < T ? max_q_len : T;
   csum::Params p;
   p.c = device_cache(cache);
   p.s = device_seqs(cache, cu_seqlens, lengths, T, max_q_len);
@@ -187,10 +194,8 @@ int weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_strid
   p.n_heads = n_heads;
   p.group = group;
   p.box = box_slots(cache->page_size, csum::TILE);
-  // the narrowest product that takes all rows of the longest sequence, 128 at most
-  const long long rows = (long long)max_q_len * group;
-  p.cols = rows >= csum::MAX_COLS ? csum::MAX_COLS : (int)((rows + 15) / 16 * 16);
-  p.toks = p.cols / group;
+  p.cols = cols;
+  p.toks = cols / group;
   p.scale_log2 = scale * kv::LOG2E;
   p.fresh = fresh;
   CUtensorMap tk, tq;
