@@ -55,3 +55,15 @@ def test_weight_sums_of_more_steps_than_are_counted_are_refused():
     kv = arg(max_pages=slots // 16, table_stride=slots // 16)
     big = dict(seq=8 * slots, head=slots, n_heads=64, T=1 << 20)
     assert sums(kv, max_q=2048, **big) == UNSUPPORTED and "too many" in _lib.load().w4a4_last_error().decode()
+
+
+def test_rotation_refuses_tables_of_negative_length_and_misaligned_offsets():
+    """Compared as an unsigned number, a negative length would let every position through."""
+    import ctypes
+    from tests.test_paged_refusals import ALIGN, BAD, P, arg, rope
+    from zip_kernel_b200 import _lib
+    L, kv = _lib.load(), arg()
+    for max_pos in (-1, -2 ** 31):
+        assert rope(kv, max_pos=max_pos, T=0) == BAD and "max_pos" in L.w4a4_last_error().decode()
+    assert L.w4a4_qkv_rope_cache(ctypes.addressof(kv), P, 48 * 128, P, P, P, P, 64, 128, None, None, 1e-6, 0, P + 2, P, 32 * 128, 128, 0, 32,
+                                 None) == ALIGN and "offsets" in L.w4a4_last_error().decode()

@@ -233,6 +233,8 @@ int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long l
   if (rc) return rc;
   CHECK_ARG(rot_dim >= 0 && rot_dim <= cache->head_dim && rot_dim % 16 == 0, "rot_dim must be a multiple of 16 up to head_dim, got %d", rot_dim);
   CHECK_ARG(rot_dim == 0 || (cos && sin), "cos or sin is NULL");
+  CHECK_ARG(max_pos >= 0, "max_pos must not be negative, got %d", max_pos);
+  if (!aligned(offsets, 4)) return fail(W4A4_ERR_ALIGNMENT, "offsets must be 4-byte aligned");
   if (T == 0 || cache->n_seqs == 0) return W4A4_OK;
   CHECK_ARG(qkv != nullptr, "qkv is NULL");
   CHECK_ARG(T == 1 || ld_qkv >= (long long)(n_heads + 2 * cache->n_kv_heads) * cache->head_dim, "ld_qkv (%lld) is below the width of a row", ld_qkv);
