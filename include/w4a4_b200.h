@@ -324,7 +324,7 @@ int w4a4_fused_dense_sparse_noalloc(const void* W_low, const void* W_high, const
  *
  * Pages: k_pages and v_pages hold n_pages pages of page_size slots (a multiple of 16) for each key/value head; element
  * (page, head, slot, d) is at page * strides[0] + head * strides[1] + slot * strides[2] + d, strides in elements,
- * positive and multiples of 8, pointers 16-byte aligned, head_dim 64 or 128.  Slot j of sequence b is slot
+ * positive, multiples of 8 and such that no slots overlap, pointers 16-byte aligned, head_dim 64 or 128.  Slot j of sequence b is slot
  * j % page_size of page block_table[b * table_stride + j / page_size].
  * Sequences: cu_seqlens (n_seqs + 1) int32 holds the first token of each sequence and the end of the last; lengths
  * (n_seqs) int32 counts the cache slots in use, those of the call's new tokens included.  New token i of sequence b

@@ -67,3 +67,27 @@ def test_rotation_refuses_tables_of_negative_length_and_misaligned_offsets():
         assert rope(kv, max_pos=max_pos, T=0) == BAD and "max_pos" in L.w4a4_last_error().decode()
     assert L.w4a4_qkv_rope_cache(ctypes.addressof(kv), P, 48 * 128, P, P, P, P, 64, 128, None, None, 1e-6, 0, P + 2, P, 32 * 128, 128, 0, 32,
                                  None) == ALIGN and "offsets" in L.w4a4_last_error().decode()
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    """Two blocks would write one place.  Strides that nest either way are taken (nothing to do: no launch)."""
+    import ctypes
+    from tests.test_paged_refusals import BAD, P, arg, attention, rope, sums
+    from zip_kernel_b200 import _lib
+    L = _lib.load()
+
+    def out(tok, head, T=3):
+        return L.w4a4_paged_attention(ctypes.addressof(arg()), P, 4096, 128, P, P, P, tok, head, None, T, 32, 1, 0.1, P, 1 << 30, None)
+
+    for tok, head in ((128, 128), (4096 - 128, 128), (128, 256), (200, 136)):
+        assert out(tok, head) == BAD and "out overlap" in L.w4a4_last_error().decode()
+        assert rope(arg(), q_tok=tok, q_head=head) == BAD and "q_out overlap" in L.w4a4_last_error().decode()
+    for seq, head in ((64, 64), (8 * 64 - 1, 64), (64, 127)):
+        assert sums(arg(), seq=seq, head=head, T=0) == BAD and "sums overlap" in L.w4a4_last_error().decode()
+    for seq, head in ((8 * 64, 64), (64, 128), (600, 70)):
+        assert sums(arg(), seq=seq, head=head, T=0) == 0
+    for st in ((8 * 16 * 128, 16 * 128, 64), (8 * 16 * 128, 128, 128), (128, 9 * 128, 9 * 8 * 64), (8 * 16 * 128 - 8, 16 * 128, 128)):
+        for kw in (dict(k_strides=st), dict(v_strides=st)):
+            assert attention(arg(**kw), T=0) == BAD and "overlap" in L.w4a4_last_error().decode()
+    for st in ((8 * 16 * 128, 128, 8 * 128), (128, 9 * 128, 9 * 8 * 128), (2 * 8 * 16 * 128, 16 * 136, 136)):
+        assert attention(arg(k_strides=st, v_strides=st), T=0) == 0

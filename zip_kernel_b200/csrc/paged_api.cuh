@@ -10,6 +10,25 @@ namespace ppre = w4a4::ppre;
 namespace csum = w4a4::csum;
 namespace evict = w4a4::evict;
 
+// Rows of `row` elements at i * s0 + j * s1, i < n0, j < n1: one of the strides covers all that the other reaches.
+bool rows_apart(long long s0, long long n0, long long s1, long long n1, long long row) {
+  if (n0 <= 1 || n1 <= 1) return (n0 <= 1 || s0 >= row) && (n1 <= 1 || s1 >= row);
+  return s0 >= s1 ? s1 >= row && s0 >= s1 * (n1 - 1) + row : s0 >= row && s1 >= s0 * (n0 - 1) + row;
+}
+
+// The same of three strides.
+bool pages_apart(const long long* st, const w4a4_paged_kv* c) {
+  struct Axis { long long stride, n; } a[3] = {{st[0], c->n_pages}, {st[1], c->n_kv_heads}, {st[2], c->page_size}};
+  std::sort(a, a + 3, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
+  long long reach = c->head_dim;
+  for (const Axis& x : a) {
+    if (x.n <= 1) continue;
+    if (x.stride < reach) return false;
+    reach += x.stride * (x.n - 1);
+  }
+  return true;
+}
+
 int check_cache(const w4a4_paged_kv* c) {
   CHECK_ARG(c != nullptr, "cache is NULL");
   CHECK_ARG(c->dtype == W4A4_F16 || c->dtype == W4A4_BF16, "cache dtype %d is neither W4A4_F16 nor W4A4_BF16", c->dtype);
@@ -27,6 +46,7 @@ int check_cache(const w4a4_paged_kv* c) {
     if (c->k_strides[i] % 8 || c->v_strides[i] % 8)
       return fail(W4A4_ERR_ALIGNMENT, "cache strides must be multiples of 8 elements");
   }
+  CHECK_ARG(pages_apart(c->k_strides, c) && pages_apart(c->v_strides, c), "slots of the cache overlap");
   if (!aligned(c->k_pages, 16) || !aligned(c->v_pages, 16) || !aligned(c->block_table, 4))
     return fail(W4A4_ERR_ALIGNMENT, "cache pointers must be 16-byte aligned");
   return W4A4_OK;
@@ -60,7 +80,7 @@ kv::Seqs device_seqs(const w4a4_paged_kv* c, const int32_t* cu, const int32_t* l
   return s;
 }
 
-// Row strides of a (T, heads, dim) operand: the heads of a token do not overlap, nor do the tokens.
+// Row strides of a (T, heads, dim) operand: the heads of a token do not overlap, nor does a head in two tokens.
 int check_rows(const char* what, const void* ptr, long long tok, long long head, int T, int n_heads, int dim) {
   CHECK_ARG(ptr != nullptr, "%s is NULL", what);
   CHECK_ARG(head >= dim || n_heads == 1, "%s: head stride %lld is below head_dim %d", what, head, dim);
@@ -168,6 +188,7 @@ int weight_sums(const w4a4_paged_kv* cache, const void* q, long long q_tok_strid
   const long long slots = (long long)cache->max_pages * cache->page_size;
   CHECK_ARG((sums_head_stride >= slots || cache->n_kv_heads == 1) && (sums_seq_stride >= slots || cache->n_seqs <= 1),
             "sums strides (%lld, %lld) are below the %lld slots of a row", sums_seq_stride, sums_head_stride, slots);
+  CHECK_ARG(slots == 0 || rows_apart(sums_seq_stride, cache->n_seqs, sums_head_stride, cache->n_kv_heads, slots), "rows of sums overlap");
   if (T == 0 || cache->n_seqs == 0 || max_q_len == 0 || slots == 0) return W4A4_OK;
   rc = check_rows("q", q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
   if (rc) return rc;
@@ -240,6 +261,7 @@ int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long l
   CHECK_ARG(T == 1 || ld_qkv >= (long long)(n_heads + 2 * cache->n_kv_heads) * cache->head_dim, "ld_qkv (%lld) is below the width of a row", ld_qkv);
   rc = check_rows("q_out", q_out, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
   if (rc) return rc;
+  CHECK_ARG(rows_apart(q_tok_stride, T, q_head_stride, n_heads, cache->head_dim), "rows of q_out overlap");
   if (!aligned(qkv, 16) || ld_qkv % 8 || !aligned(cos, 16) || !aligned(sin, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16))
     return fail(W4A4_ERR_ALIGNMENT, "qkv, cos, sin and the norm weights must be 16-byte aligned");
   DeviceInfo* dev = nullptr;
@@ -305,6 +327,7 @@ int w4a4_paged_attention(const w4a4_paged_kv* cache, const void* q, long long q_
   rc = check_rows("q", q, q_tok_stride, q_head_stride, T, n_heads, cache->head_dim);
   if (!rc) rc = check_rows("out", out, out_tok_stride, out_head_stride, T, n_heads, cache->head_dim);
   if (rc) return rc;
+  CHECK_ARG(rows_apart(out_tok_stride, T, out_head_stride, n_heads, cache->head_dim), "rows of out overlap");
   if (!aligned(lse, 4)) return fail(W4A4_ERR_ALIGNMENT, "lse must be 4-byte aligned");
   DeviceInfo* dev = nullptr;
   rc = current_device(&dev);
