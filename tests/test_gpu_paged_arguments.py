@@ -37,3 +37,24 @@ def test_sequences_without_any_page_need_no_earlier_call():
                                                 max_q_len=q_len, return_lse=True)
         assert (out[:q_len + 1] == 0).all() and (lse[:q_len + 1] == float("-inf")).all()
     assert _lib.device_error(DEV) == 0
+
+
+@pytest.mark.parametrize("length,written", [(97, [0, 1]), (98, [0]), (99, []), (200, []), (2 ** 31 - 1, []), (-1, []), (-2 ** 31, []), (2, [1, 2])])
+def test_tokens_beyond_the_table_take_no_other_slot(length, written):
+    """Sequence 1 has three new tokens and six pages of 16 slots: those whose slot exists are written there, the others nowhere."""
+    from zip_kernel_b200 import _lib, ops
+    c = R.Case([1, 3], [50, 96], 8, 2, 128, 16, "fp16", seed=35, max_pages=6)
+    cos = torch.ones(256, 64, device=DEV)
+    sin = torch.zeros(256, 64, device=DEV)
+    kv, n = c.kv(), torch.tensor([50, length], dtype=torch.int32, device=DEV)
+    want_k, want_v = c.k.clone(), c.v.clone()
+    rows = c.qkv.view(4, 12, 128)
+    for t, slot in [(0, 49)] + [(1 + i, length - 3 + i) for i in written]:
+        b = min(t, 1)
+        page, at = int(c.table[b, slot // 16]), slot % 16
+        want_k[page, :, at], want_v[page, :, at] = rows[t, 8:10], rows[t, 10:12]
+    _lib.device_error(DEV)
+    ops.qkv_rope_cache_cuda(c.qkv.to(DEV), kv, c.cu.to(DEV), n, cos, sin)
+    assert _lib.device_error(DEV) != 0
+    assert torch.equal(kv.k_pages.cpu().nan_to_num(9.0), want_k.nan_to_num(9.0))
+    assert torch.equal(kv.v_pages.cpu().nan_to_num(9.0), want_v.nan_to_num(9.0))

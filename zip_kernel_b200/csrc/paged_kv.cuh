@@ -39,9 +39,10 @@ struct Seq {
   int q0, q_len, len;
 };
 
-// Reads sequence b.  What cannot be true is cut to what can and reported.
-__device__ __forceinline__ Seq load_seq(const Seqs& s, int b) {
-  const int c0 = ld_plain(s.cu + b), c1 = ld_plain(s.cu + b + 1), n = ld_plain(s.lengths + b);
+// Reads sequence b.  What cannot be true is cut to what can and reported; `n` is the length as it was given.
+__device__ __forceinline__ Seq load_seq(const Seqs& s, int b, int& n) {
+  const int c0 = ld_plain(s.cu + b), c1 = ld_plain(s.cu + b + 1);
+  n = ld_plain(s.lengths + b);
   Seq r;
   r.q0 = min(max(c0, 0), s.T);
   r.q_len = min(max(c1, r.q0), s.T) - r.q0;
@@ -49,6 +50,10 @@ __device__ __forceinline__ Seq load_seq(const Seqs& s, int b) {
   if (r.q0 != c0 || r.q0 + r.q_len != c1 || r.len != n || r.q_len > s.max_q) record_error(SITE_KV_SEQ, b);
   r.q_len = min(r.q_len, s.max_q);
   return r;
+}
+__device__ __forceinline__ Seq load_seq(const Seqs& s, int b) {
+  int n;
+  return load_seq(s, b, n);
 }
 
 // Page number of `slot` of sequence b, or -1 (reported) when the table holds none of the cache's.

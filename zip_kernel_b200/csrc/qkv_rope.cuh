@@ -97,8 +97,11 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) qkv_rope_kernel(const RopePar
   for (int i = lane; i <= p.s.n; i += 32) below += ld_plain(p.s.cu + i) <= t;
   const int b = __reduce_add_sync(0xffffffffu, below) - 1;
   if (b < 0 || b >= p.s.n) return;           // behind the last sequence: left as it is
-  const Seq q = load_seq(p.s, b);
-  const int slot = q.len - q.q_len + (t - q.q0);
+  int length;
+  const Seq q = load_seq(p.s, b, length);
+  // from the length as it was given: a token of a sequence that has outgrown its table must not take an earlier one's slot
+  const long long at = (long long)length - q.q_len + (t - q.q0);
+  const int slot = at >= 0 && at < p.s.max_slots ? (int)at : -1;
   const int pos = slot + (p.offsets ? ld_plain(p.offsets + b) : 0);
   if (slot < 0 || (p.rot > 0 && (unsigned)pos >= (unsigned)p.max_pos) || t < q.q0 || t >= q.q0 + q.q_len) {
     if (lane == 0) record_error(SITE_KV_POS, b);
