@@ -150,18 +150,22 @@ struct AttnPlan {
   int toks;                   // tokens of a row tile of the latter
   size_t few_parts, many_parts, joins, total;
 };
-// A sequence with up to this many rows (new tokens x heads of a group) goes to the kernel for few rows: two row tiles of it,
-// the second of which finds keys and values in L2.  Measured, few against many rows: 32 sequences up to 4096 slots, 20
-// rows 59 to 90 us, 32 rows 83 to 103; 8 up to 32768, 32 rows 125 to 139; one of 8191, 32 rows 27 to 33; but 64 rows
-// 145 to 114, 236 to 168 and 37 to 33.
-constexpr int ATTN_FEW_ROWS = 2 * pdec::ROWS;
+// A sequence with up to this many rows (new tokens x heads of a group) goes to the kernel for few rows: one row tile of it
+// where there are many (sequence, key/value head) pairs, else two, the second of which reads keys and values again.  The
+// kernel for many rows reads them once but has three launches.  Measured at 8 key/value heads, dim 128, few against many
+// rows, with 20 and with 32 rows: one history of 8191 24 to 29 us, 26 to 29; 2 up to 8191 24 to 30, 26 to 31; 4 40 to 42, 42 to 41;
+// 8 64 to 55, 80 to 55; 32 178 to 145, 214 to 142; 4 up to 512 15 to 20, 16 to 20; 8 21 to 21, 27 to 21; 64 62 to 52, 79 to 53.
+constexpr int ATTN_MANY_PAIRS = 64;
+int attn_few_rows(const w4a4_paged_kv* c) {
+  return (long long)c->n_seqs * c->n_kv_heads >= ATTN_MANY_PAIRS ? pdec::ROWS : 2 * pdec::ROWS;
+}
 
 AttnPlan attn_plan(const w4a4_paged_kv* c, int T, int n_heads, int max_q, int sm_count) {
   AttnPlan a{};
-  const int group = n_heads / c->n_kv_heads;
-  a.many = (long long)max_q * group > ATTN_FEW_ROWS && group <= ppre::ROWS;
+  const int group = n_heads / c->n_kv_heads, few_rows = attn_few_rows(c);
+  a.many = (long long)max_q * group > few_rows && group <= ppre::ROWS;
   a.few = !a.many || c->n_seqs > 1;                        // one sequence: whatever its length, one kernel
-  a.few_rows = !a.many ? 0x7fffffff : a.few ? ATTN_FEW_ROWS : 0;
+  a.few_rows = !a.many ? 0x7fffffff : a.few ? few_rows : 0;
   a.toks = a.many ? ppre::ROWS / group : 0;
   size_t off = W4A4_ATTENTION_STATE_BYTES;
   a.few_parts = off;

@@ -230,7 +230,8 @@ def paged_attention_cuda(q: torch.Tensor, kv: PagedKV, cu_seqlens: torch.Tensor,
     logarithm of each row's sum of exponentials.
 
     ``scale``: of the scores, ``head_dim ** -0.5`` by default.  ``max_q_len``: no sequence has more new tokens (``T`` by
-    default); pass 1 for a decode step, so that only the kernel for few rows is launched.  A row that sees no slot is
+    default); pass 1 for a decode step, so that with up to 16 heads on a key/value head only the kernel for few rows is
+    launched.  A row that sees no slot is
     zero, its ``lse`` minus infinity.  ``out`` may be ``q``.  Tokens behind the last sequence are left as ``out`` holds them (undefined without
     ``out``, like their ``lse``).  Values within a sequence's length must be finite; what lies behind it does not matter."""
     q, T, n_heads, tok, head = _query_rows(kv, q)
