@@ -324,14 +324,16 @@ int w4a4_fused_dense_sparse_noalloc(const void* W_low, const void* W_high, const
  *
  * Pages: k_pages and v_pages hold n_pages pages of page_size slots (a multiple of 16) for each key/value head; element
  * (page, head, slot, d) is at page * strides[0] + head * strides[1] + slot * strides[2] + d, strides in elements,
- * positive, multiples of 8 and such that no slots overlap, pointers 16-byte aligned, head_dim 64 or 128.  Slot j of sequence b is slot
- * j % page_size of page block_table[b * table_stride + j / page_size].
+ * positive, multiples of 8 and such that no slots overlap, pointers 16-byte aligned, head_dim 64 or 128.  Slot j of
+ * sequence b is slot j % page_size of page block_table[b * table_stride + j / page_size]; the rows of the table lie apart
+ * (table_stride >= max_pages).  Outputs are rows that do not overlap.
  * Sequences: cu_seqlens (n_seqs + 1) int32 holds the first token of each sequence and the end of the last; lengths
  * (n_seqs) int32 counts the cache slots in use, those of the call's new tokens included.  New token i of sequence b
  * has slot lengths[b] - q_len[b] + i and sees the slots up to its own.  Both are device memory, like block_table, and
  * no host check sees their values: what is out of range (a page number, a length beyond max_pages * page_size, offsets
  * that do not rise, more new tokens than max_q_len, a position outside the tables) is cut to what is in range, reads
- * zeros or is left out, and sets the device error word (w4a4_device_error).  A sequence may have no new token; tokens
+ * zeros or is left out (a new token without a slot is not written anywhere), and sets the device error word
+ * (w4a4_device_error).  A sequence may have no new token; tokens
  * behind the last sequence are neither read nor written. */
 #define W4A4_F16  0
 #define W4A4_BF16 1
@@ -361,7 +363,9 @@ int w4a4_qkv_rope_cache(const w4a4_paged_kv* cache, const void* qkv, long long l
  * h / (n_heads / n_kv_heads).  A token that sees no slot (its own would be negative) gets zeros.  lse (T, n_heads)
  * float, or NULL: natural logarithm of the sum of exponentials, minus infinity where nothing is seen.  Values in slots
  * that a token does not see must be finite up to its sequence's length (a weight of zero times infinity is NaN);
- * beyond the length they may hold anything.  max_q_len: no sequence has more new tokens.
+ * beyond the length they may hold anything.  max_q_len: no sequence has more new tokens.  Scores, sums and outputs are
+ * carried in float.  Of a sequence with few rows (new tokens x heads that share a key/value head: up to 16, or 32 where
+ * n_seqs * n_kv_heads is below 64) only the output is rounded to 16 bits; of one with more rows a weight is too.
  * workspace: w4a4_paged_attention_workspace_bytes (0: an argument is bad), 16-byte aligned; its first
  * W4A4_ATTENTION_STATE_BYTES must be zero before the first call and are zero again after each; calls that share it
  * must be ordered on one stream, from whatever threads: the launches of a call stay together there.  It is not the

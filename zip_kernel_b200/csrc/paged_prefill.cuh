@@ -21,8 +21,9 @@
 // What bounds it: products and exponentials alike at dim 128, 2048 clocks each per step of both row tiles if each had the SM to
 // itself.  A row tile's own chain is longer - scores read 100, maximum 400, weights 1300 to 1500 beside the other tile's,
 // then the hand-over and its products - and tensor memory is full (scores and outputs of both row tiles), so the next
-// scores cannot be made ahead: a step takes about 3200 clocks.  Measured: 8192-token prompt, 32/8 heads, 491 us, 1120
-// TFLOP/s.  One thread issues the products of both row tiles, in turn: with a thread for each the two fall into step and
+// scores cannot be made ahead: a step takes about 3200 clocks.  Measured: 8192-token prompt, 32/8 heads, 495 us, 1110
+// TFLOP/s at 1965 MHz (60 calls in a row); 569 us in a row of seconds, in which the power limit holds the clock at 1627 MHz.
+// One thread issues the products of both row tiles, in turn: with a thread for each the two fall into step and
 // no longer fill each other's pauses (607 us).
 #pragma once
 
