@@ -49,3 +49,19 @@ def test_evict_from_long_histories(lens, kv_heads, budget, sink, recent, kind, w
     assert torch.equal(got[2].cpu()[..., :budget].nan_to_num(123.0), new_sums.nan_to_num(123.0)) and not got[2][..., budget:].any()
     assert torch.equal((into or kv).k_pages.cpu(), want_k) and torch.equal((into or kv).v_pages.cpu(), want_v)
     assert _lib.device_error(DEV) == 0
+
+
+def test_fresh_sums_of_the_longest_table_are_written_whole():
+    """2^31 - 2048 slots a row, eight in use: zeros behind them all the same."""
+    from zip_kernel_b200 import _lib, ops
+    slots = 2 ** 31 - 2048
+    k = torch.randn(1, 1, 16, 64, generator=torch.Generator().manual_seed(52)).half().to(DEV)
+    kv = ops.PagedKV(k, k, torch.zeros(1, slots // 16, dtype=torch.int32, device=DEV))
+    q, cu = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(53)).half().to(DEV), torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    n = torch.tensor([8], dtype=torch.int32, device=DEV)
+    _, lse = ops.paged_attention_cuda(q, kv, cu, n, max_q_len=1, return_lse=True)
+    sums = torch.full((1, 1, slots), float("nan"), device=DEV)
+    assert _lib.load().w4a4_cache_weight_sums_fresh(kv._ptr, q.data_ptr(), 128, 64, cu.data_ptr(), n.data_ptr(), lse.data_ptr(), sums.data_ptr(),
+                                                    slots, slots, 1, 2, 1, 0.125, _lib.stream_ptr(DEV)) == 0
+    small = ops.cache_weight_sums_cuda(q, ops.PagedKV(k, k, torch.zeros(1, 1, dtype=torch.int32, device=DEV)), cu, n, lse)
+    assert torch.equal(sums[..., :16], small) and not sums[..., 16:].any() and _lib.device_error(DEV) == 0

@@ -82,7 +82,7 @@ struct Part {
 // heads, 31 us; 33 with a launch before that zeroes all of sums.
 __device__ __forceinline__ void zero_rest(const Params& p) {
   constexpr int CHUNK = 4096;
-  const int n_chunks = (p.s.max_slots + CHUNK - 1) / CHUNK;
+  const int n_chunks = (p.s.max_slots - 1) / CHUNK + 1;      // (there is a slot, and up to 2^31 - 1025 of them)
   const long long all = (long long)p.s.n * p.c.n_kv * n_chunks;
   for (long long i = blockIdx.x; i < all; i += gridDim.x) {
     const int row = (int)(i / n_chunks), c0 = (int)(i - (long long)row * n_chunks) * CHUNK, b = row / p.c.n_kv;
