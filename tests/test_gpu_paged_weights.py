@@ -95,3 +95,20 @@ def test_weights_of_few_rows_are_not_rounded_to_the_type(news, lens, heads, kv_h
     # the scale's rounding and the exponentials, the additions
     rel = u * u + 2.0 ** -21 * (1 + mag) + (max(lens) + 16) * 2.0 ** -24
     R.assert_within(out, ref, u * ref.abs() + 1.01 * rel[..., None] * (amp + ref.abs()) + 2.0 ** -25, "out")
+
+
+@pytest.mark.parametrize("news,lens,heads,kv_heads", [
+    ([4, 5, 8, 9, 1, 0, 3, 6], [300, 5, 130, 700, 64, 40, 3, 257], 32, 8),       # 16 rows and fewer, 20, 32, 36 side by side
+    ([1] * 64, [1 + (37 * b) % 400 for b in range(64)], 24, 1),                  # 24 rows of one token each
+    ([8, 4], [500, 333], 16, 4), ([5] * 15, [20 + 31 * b for b in range(15)], 16, 4),      # fewer than 64 pairs
+])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_sequences_on_both_sides_of_the_border(news, lens, heads, kv_heads, dtype):
+    from zip_kernel_b200 import _lib, ops
+    c = R.Case(news, lens, heads, kv_heads, 64, 16, dtype, seed=25, q_scale=2.0)
+    ref, ref_lse, amp, mag = R.attention_ref(c)
+    for max_q in (max(news), None):
+        out, lse = ops.paged_attention_cuda(c.q.to(DEV), c.kv(), c.cu.to(DEV), c.lengths.to(DEV), max_q_len=max_q, return_lse=True)
+        R.assert_within(out, ref, R.attention_tolerance(c, ref, amp, mag), "out")
+        R.assert_within(lse, ref_lse, R.lse_tolerance(c, ref_lse, mag), "lse")
+    assert _lib.device_error(DEV) == 0
